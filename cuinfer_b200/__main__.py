@@ -39,6 +39,7 @@ def main(argv=None) -> int:
     g.add_argument("--top-p", type=float, default=1.0)
     g.add_argument("--ignore-eos", action="store_true")
     g.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    g.add_argument("--kv-cache-dtype", choices=["auto", "int4"], default="auto", help="how keys and values are held: in the model's dtype, or in 4 bits")
     g.add_argument("--gpu-memory-utilization", type=float, default=0.8)
     g.add_argument("--block-size", type=int, default=16)
     g.add_argument("--num-blocks", type=int, default=None, help="cache pages; default: from free memory")
@@ -62,7 +63,7 @@ def main(argv=None) -> int:
         options = dict(gpu_memory_utilization=args.gpu_memory_utilization, block_size=args.block_size,
                        max_num_scheduled_tokens=args.max_num_scheduled_tokens, max_num_seqs=args.max_num_seqs,
                        enable_cuda_graph=not args.disable_cuda_graph, decode_run_ahead=not args.disable_run_ahead, dtype=args.dtype, num_blocks=args.num_blocks,
-                       seed=args.seed)
+                       seed=args.seed, kv_cache_dtype=args.kv_cache_dtype)
         EngineConfig(model_path=args.model or "", **options)
         params = SamplingParams(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
                                 max_tokens=args.max_tokens, ignore_eos=args.ignore_eos)

@@ -1,0 +1,190 @@
+// Paged causal attention over the cache that is held in 4 bits (kv4.cuh), the all-sizes kernel: any head size that is a
+// multiple of 32 up to 256, any head counts, 32-bit or bfloat16 queries, an optional window.
+//
+//   out = softmax(scale * q K^T over the keys position - window < j <= position) V
+//
+// The queries of a request are the last n positions of its sequence.  A CTA takes one token and up to four query heads of one kv
+// head (a key is taken apart once for all four); its warps share the keys in chunks of 32, a key to a lane for the scores, a value
+// column to a lane for the weighted sum, and merge their running maxima and sums in shared memory.  32-bit throughout,
+// the exact exponential; nothing is rounded before the end.  Keys whose page the block table does not name are left out; a row
+// without keys is zero; rows that belong to no request are left as they are.
+#include "kv4.cuh"
+#include "mma_utils.cuh"
+
+namespace cib {
+namespace kv4 {
+
+constexpr int kHeads = 4;
+constexpr int kMaxWarps = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(kMaxWarps * 32)
+attention_generic_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out, int out_stride, unsigned char* __restrict__ cache, int num_pages,
+                         int page_size, const int* __restrict__ block_table, int table_stride, const int* __restrict__ query_start_loc,
+                         const int* __restrict__ seq_lens, int num_requests, int least_query, int nq, int nkv, int d, float scale, int window) {
+    extern __shared__ float smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int t = blockIdx.x, kvh = blockIdx.y;
+    const int g = nq / nkv;
+    const int head0 = kvh * g + blockIdx.z * kHeads;
+    const int nh = min(kHeads, (kvh + 1) * g - head0);
+    const int groups = d / kGroup;
+    griddep_wait();
+    griddep_launch();
+    // the request of this row: the last one that starts at or before it
+    int before = 0;
+    for (int r0 = 0; r0 <= num_requests; r0 += 32) {
+        const int r = r0 + lane;
+        before += __popc(__ballot_sync(0xffffffffu, r <= num_requests && query_start_loc[min(r, num_requests)] <= t));
+    }
+    const int r = before - 1;
+    if (r < 0 || r >= num_requests) return;
+    const int q0 = query_start_loc[r], n = query_start_loc[r + 1] - q0;
+    if (n < least_query) return;
+    const int pos = seq_lens[r] - n + (t - q0);
+    const int lo = window > 0 ? max(0, pos - window + 1) : 0;
+    const int* table = block_table + (size_t)r * table_stride;
+
+    float* qs = smem;                                      // [head][d], scaled
+    for (int i = threadIdx.x; i < nh * d; i += blockDim.x) qs[i] = to_f32(q[(size_t)t * q_stride + (size_t)head0 * d + i]) * scale;
+    __syncthreads();
+
+    float acc[kHeads][kMaxHeadDim / kGroup];
+    float m[kHeads], l[kHeads];
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+        m[h] = -INFINITY, l[h] = 0.f;
+#pragma unroll
+        for (int k = 0; k < kMaxHeadDim / kGroup; ++k) acc[h][k] = 0.f;
+    }
+    for (int c = lo + warp * 32; c <= pos; c += warps * 32) {
+        const int j = c + lane;
+        const unsigned char* block = nullptr;
+        if (j <= pos && j / page_size < table_stride) {
+            const int page = table[j / page_size];
+            if (page >= 0 && page < num_pages) block = block_of(cache, page * page_size + j % page_size, num_pages, page_size, nkv, kvh, d);
+        }
+        float s[kHeads];
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) s[h] = block != nullptr ? 0.f : -INFINITY;
+        if (block != nullptr) {
+            const uint32_t* codes = reinterpret_cast<const uint32_t*>(block) + (j % kBlock) * 4 * groups;
+            const uint16_t* words = reinterpret_cast<const uint16_t*>(block + key_words_at(d)) + (j % kBlock) * groups;
+            for (int k = 0; k < groups; ++k) {
+                const uint32_t w = words[k];
+                const int zero = (int)(w & 15u);
+                float dot[kHeads] = {0.f, 0.f, 0.f, 0.f};
+                for (int u = 0; u < 4; ++u) {
+                    const uint32_t code = codes[u * groups + k];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float x = (float)((int)((code >> (4 * (e >> 1) + 16 * (e & 1))) & 15u) - zero);
+#pragma unroll
+                        for (int h = 0; h < kHeads; ++h)
+                            if (h < nh) dot[h] = fmaf(qs[h * d + k * kGroup + u * 8 + e], x, dot[h]);
+                    }
+                }
+                const float step = step_of(w);
+#pragma unroll
+                for (int h = 0; h < kHeads; ++h) s[h] = fmaf(step, dot[h], s[h]);
+            }
+        }
+        float p[kHeads];
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+            const float top = fmaxf(m[h], warp_max(s[h]));
+            const float base = top == -INFINITY ? 0.f : top;
+            p[h] = block != nullptr ? expf(s[h] - base) : 0.f;
+            const float corr = m[h] == -INFINITY ? 0.f : expf(m[h] - base);
+            l[h] = l[h] * corr + warp_sum(p[h]);
+            m[h] = top;
+#pragma unroll
+            for (int k = 0; k < kMaxHeadDim / kGroup; ++k) acc[h][k] *= corr;
+        }
+        const int count = min(32, pos - c + 1);
+        for (int jj = 0; jj < count; ++jj) {
+            const unsigned char* from = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, (unsigned long long)block, jj));
+            float pj[kHeads];
+#pragma unroll
+            for (int h = 0; h < kHeads; ++h) pj[h] = __shfl_sync(0xffffffffu, p[h], jj);
+            if (from == nullptr) continue;
+            const int token = (c + jj) % kBlock;
+            const uint16_t* words = reinterpret_cast<const uint16_t*>(from + value_words_at(d)) + (token >> 1) * groups * 2 + (token & 1);
+            const uint16_t* codes = reinterpret_cast<const uint16_t*>(from + value_codes_at(d)) +
+                                    (size_t)(((token >> 3) * 8 + (lane >> 2)) * 4 + ((token & 7) >> 1)) * groups * 2 + (token & 1);
+#pragma unroll
+            for (int k = 0; k < kMaxHeadDim / kGroup; ++k) {
+                if (k < groups) {
+                    const uint32_t w = words[2 * k];
+                    const float x = step_of(w) * (float)((int)((codes[2 * k] >> (4 * (lane & 3))) & 15u) - (int)(w & 15u));
+#pragma unroll
+                    for (int h = 0; h < kHeads; ++h) acc[h][k] = fmaf(pj[h], x, acc[h][k]);
+                }
+            }
+        }
+    }
+    // merge: [warp][head][d + 2]
+    float* part = smem + kHeads * d;
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+        float* mine = part + (size_t)(warp * kHeads + h) * (d + 2);
+#pragma unroll
+        for (int k = 0; k < kMaxHeadDim / kGroup; ++k)
+            if (k < groups) mine[k * kGroup + lane] = acc[h][k];
+        if (lane == 0) mine[d] = m[h], mine[d + 1] = l[h];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < nh * d; i += blockDim.x) {
+        const int h = i / d, x = i - h * d;
+        float top = -INFINITY, sum = 0.f, o = 0.f;
+        for (int w = 0; w < warps; ++w) top = fmaxf(top, part[(size_t)(w * kHeads + h) * (d + 2) + d]);
+        for (int w = 0; w < warps; ++w) {
+            const float* from = part + (size_t)(w * kHeads + h) * (d + 2);
+            const float f = from[d] == -INFINITY ? 0.f : expf(from[d] - top);
+            sum += from[d + 1] * f;
+            o += from[x] * f;
+        }
+        // (a sum that is not a number stays one: only a row without keys is zero)
+        out[(size_t)t * out_stride + (size_t)head0 * d + i] = from_f32<T>(sum == 0.f ? 0.f : o / sum);
+    }
+}
+
+}  // namespace kv4
+}  // namespace cib
+
+using namespace cib;
+
+// query_start_loc holds num_requests + 1 boundaries of the num_tokens rows.  longest: no request has more keys (it shapes the launch only).
+// least_query: rows of requests that bring fewer tokens are left as they are.
+extern "C" int cib_attention_kv4_generic(const void* q, int dtype, int q_stride, void* out, int out_stride, const void* cache, int num_pages, int page_size,
+                                         const int* block_table, int table_stride, const int* query_start_loc, const int* seq_lens, int num_tokens,
+                                         int num_requests, int longest, int least_query, int nq, int nkv, int d, float scale, int window, int use_pdl,
+                                         cudaStream_t stream) {
+    CIB_REQUIRE(num_tokens >= 0 && nq > 0 && nkv > 0 && nq % nkv == 0, "attention_kv4: bad sizes T=%d nq=%d nkv=%d", num_tokens, nq, nkv);
+    CIB_REQUIRE(kv4::sizes_ok(d, page_size), "attention_kv4: head size %d must be a multiple of 32 up to 256, page size %d a multiple of 16", d, page_size);
+    CIB_REQUIRE(num_requests > 0 || num_tokens == 0, "attention_kv4: tokens without requests");
+    CIB_REQUIRE(num_pages > 0 && table_stride > 0 && cache != nullptr && ((uintptr_t)cache % 16) == 0, "attention_kv4: bad cache geometry");
+    CIB_REQUIRE((long long)num_pages * page_size < (1ll << 31), "attention_kv4: %d pages of %d slots do not fit 32-bit slot numbers", num_pages, page_size);
+    CIB_REQUIRE(q_stride >= nq * d && out_stride >= nq * d, "attention_kv4: row strides %d and %d are too small", q_stride, out_stride);
+    CIB_REQUIRE(window >= 0, "attention_kv4: window must be >= 0 (0 = all keys)");
+    CIB_REQUIRE(dtype == kF32 || dtype == kBF16, "attention_kv4: unsupported dtype %d", dtype);
+    const int g = nq / nkv;
+    CIB_REQUIRE(nkv <= 65535 && (g + kv4::kHeads - 1) / kv4::kHeads <= 65535, "attention_kv4: too many heads");
+    if (num_tokens == 0) return 0;
+    // a warp for every two chunks of 32 keys, so that a short context's merge stays small
+    const int keys = window > 0 && window < longest ? window : longest;
+    const int warps = keys <= 64 ? 1 : keys <= 128 ? 2 : keys <= 512 ? 4 : kv4::kMaxWarps;
+    const size_t smem = (size_t)(kv4::kHeads * d + warps * kv4::kHeads * (d + 2)) * sizeof(float);
+    const dim3 grid(num_tokens, nkv, (g + kv4::kHeads - 1) / kv4::kHeads);
+    cudaError_t e;
+    if (dtype == kF32)
+        e = launch_pdl(kv4::attention_generic_kernel<float>, grid, dim3(warps * 32), smem, stream, use_pdl != 0, (const float*)q, q_stride, (float*)out, out_stride,
+                       (unsigned char*)cache, num_pages, page_size, block_table, table_stride, query_start_loc, seq_lens, num_requests, least_query, nq, nkv, d,
+                       scale, window);
+    else
+        e = launch_pdl(kv4::attention_generic_kernel<__nv_bfloat16>, grid, dim3(warps * 32), smem, stream, use_pdl != 0, (const __nv_bfloat16*)q, q_stride,
+                       (__nv_bfloat16*)out, out_stride, (unsigned char*)cache, num_pages, page_size, block_table, table_stride, query_start_loc, seq_lens,
+                       num_requests, least_query, nq, nkv, d, scale, window);
+    CIB_REQUIRE(e == cudaSuccess, "attention_kv4: launch failed: %s", cudaGetErrorString(e));
+    return 0;
+}

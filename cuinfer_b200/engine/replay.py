@@ -28,7 +28,7 @@ TRACE_TOKEN_ROUNDING = 64
 
 
 def make_runner(model_dir: str, dtype: str, max_tokens: int, block_size: int = 16, max_live: int = 4,
-                cuda_graph: bool = False) -> ModelRunner:
+                cuda_graph: bool = False, kv_cache_dtype: str = "auto") -> ModelRunner:
     """A runner whose page pool holds exactly ``max_tokens`` tokens (rounded up to whole pages).
     ``cuda_graph``: steps go the way generation sends them — a step of single tokens that all want their logits
     through ``ModelRunner.decode_step`` (one CUDA graph per bucket of rows and class of context length), a
@@ -40,7 +40,8 @@ def make_runner(model_dir: str, dtype: str, max_tokens: int, block_size: int = 1
     rounded = (max_tokens + unit - 1) // unit * unit
     pages = (rounded + block_size - 1) // block_size
     config = EngineConfig(model_path=model_dir, block_size=block_size, dtype=dtype, num_blocks=pages,
-                          max_num_seqs=max_live, max_num_scheduled_tokens=1 << 30, enable_cuda_graph=cuda_graph)
+                          max_num_seqs=max_live, max_num_scheduled_tokens=1 << 30, enable_cuda_graph=cuda_graph,
+                          kv_cache_dtype=kv_cache_dtype)
     return ModelRunner(model_dir, config)
 
 
@@ -91,8 +92,9 @@ def main(argv: Optional[List[str]] = None) -> int:
     parser.add_argument("--block-size", type=int, default=16, help="tokens per cache page")
     parser.add_argument("--graphs", action="store_true",
                         help="run decode steps and steps whose bucket of sizes has come before from CUDA graphs, as generation does")
+    parser.add_argument("--kv-cache-dtype", choices=["auto", "int4"], default="auto", help="how keys and values are held")
     args = parser.parse_args(argv)
-    runner = make_runner(args.model, args.dtype, args.max_tokens, args.block_size, cuda_graph=args.graphs)
+    runner = make_runner(args.model, args.dtype, args.max_tokens, args.block_size, cuda_graph=args.graphs, kv_cache_dtype=args.kv_cache_dtype)
     run_trace(runner, sys.stdin, args.out)
     return 0
 

@@ -23,7 +23,7 @@ import numpy as np
 import torch
 
 from ..cache import CacheManager, CacheStorage, group_runs, page_bytes
-from ..config import EngineConfig, load_model_config
+from ..config import ConfigError, EngineConfig, load_model_config
 from ..parts import DecoderModel, GroupView, PagedKV, StepContext
 from ..weights import open_weight_store
 
@@ -91,13 +91,19 @@ class ModelRunner:
 
         needs = self.model.cache_needs()
         self.groups = group_runs(needs)
+        self.kv4 = config.kv_cache_dtype == "int4"
+        if self.kv4:
+            for run in needs:
+                if not self.model.blocks[self.model.order[run]].mixer.takes_kv4(self.page_size):
+                    raise ConfigError(f"kv_cache_dtype 'int4': the attention of layer {self.model.order[run]} does not take a cache in "
+                                      "4 bits (grouped-query attention with a head size that is a multiple of 32 up to 256 does)")
         pages = num_blocks if num_blocks is not None else config.num_blocks
         if pages is None:
             pages = self._pages_from_memory()
         self.num_pages = int(pages)
         self.manager = CacheManager(self.groups, self.page_size, self.num_pages, config.max_num_seqs)
         self.storage = CacheStorage(self.groups, self.page_size, [self.num_pages] * len(self.groups),
-                                    self.model.state_needs(), config.max_num_seqs, self.dtype, self.device)
+                                    self.model.state_needs(), config.max_num_seqs, self.dtype, self.device, kv4=self.kv4)
         # which cache every run uses (its own, or an earlier run's)
         self._run_cache: Dict[int, tuple[int, bool]] = {}
         for run, _layer in self.model.runs():
@@ -122,7 +128,7 @@ class ModelRunner:
 
     # ---- sizing ------------------------------------------------------------------------------------
     def page_bytes(self) -> int:
-        return sum(page_bytes(g, self.page_size, self.dtype) for g in self.groups)
+        return sum(page_bytes(g, self.page_size, self.dtype, self.kv4) for g in self.groups)
 
     def _pages_from_memory(self) -> int:
         """Pages that fit in ``gpu_memory_utilization`` of the device after the weights

@@ -119,6 +119,9 @@ def _declare(lib: ctypes.CDLL) -> None:
         "cib_paged_attention_decode": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _F, _I, _I, _P, _P, _I, _P, _P, ctypes.c_longlong, _P],
         "cib_paged_attention_prefill": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _P],
         "cib_attention_tcgen05": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P],
+        "cib_qk_norm_rope_kv4_write": [_P, _I, _I, _P, _I, _P, _P, _P, _P, _I, _I, _F, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P],
+        "cib_kv4_read": [_P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
+        "cib_attention_kv4_generic": [_P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
         "cib_gemm_skinny": [_P, _I, _I, _I, _P, _I, _P, _P, _I, _P, _I, _F, _P, _P, _I, _I, _I, _I, _I, _P, ctypes.c_longlong, _P, _I, _P, _P, _P],
         "cib_gemm_tcgen05": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P, _I, _F, _P, _P, _I, _P, _P, _P],
         "cib_gemm_wstream": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _P, _I, _F, _P, _P, _I, _P, _P, _I, _P, ctypes.c_longlong, _I, _P, _P],
@@ -740,6 +743,150 @@ def paged_attention_prefill(q: torch.Tensor, out: torch.Tensor, cache: torch.Ten
         _cuda(seq_lens, "seq_lens", torch.int32), len(query_lens_host), tiles, num_q_heads, num_kv_heads, head_dim,
         float(scale), int(window), pair, _stream())
     _check(rc, "paged_attention_prefill")
+    _count()
+
+
+# ---- the cache held in 4 bits --------------------------------------------------------------------------
+
+KV4_GROUP = 32       # neighbouring values of a head that share a step and a zero point
+KV4_BLOCK = 16       # tokens of a cache block
+KV4_MAX_HEAD_DIM = 256
+
+
+def kv4_supports(head_dim: int, page_size: int) -> bool:
+    """Whether the cache can be held in 4 bits: whole groups in a head, whole blocks in a page."""
+    return 0 < head_dim <= KV4_MAX_HEAD_DIM and head_dim % KV4_GROUP == 0 and page_size > 0 and page_size % KV4_BLOCK == 0
+
+
+def kv4_cache_shape(num_pages: int, num_kv_heads: int, page_size: int, head_dim: int) -> tuple:
+    """The shape of the uint8 tensor that holds ``num_pages`` pages of keys and values in 4 bits: 18 * head_dim bytes a block of 16
+    tokens (4.5 bits a value).  A page id stands for the same tokens as in a cache of 16- or 32-bit numbers.  Fresh pages may hold
+    anything: what no token has been written to is not read."""
+    if not kv4_supports(head_dim, page_size):
+        raise KernelError(f"a cache in 4 bits needs a head size that is a multiple of {KV4_GROUP} up to {KV4_MAX_HEAD_DIM} and pages of a "
+                          f"multiple of {KV4_BLOCK} slots, got head size {head_dim}, pages of {page_size}")
+    return (num_pages, num_kv_heads, page_size // KV4_BLOCK, 18 * head_dim)
+
+
+def _kv4_cache(cache: torch.Tensor, num_kv_heads: int, head_dim: int, who: str) -> int:
+    """Checks the cache; its page size."""
+    if cache.dtype != torch.uint8 or cache.dim() != 4 or cache.shape[1] != num_kv_heads or cache.shape[3] != 18 * head_dim:
+        raise KernelError(f"{who}: cache must be uint8 [pages, {num_kv_heads}, page_size / {KV4_BLOCK}, {18 * head_dim}], got "
+                          f"{cache.dtype} {list(cache.shape)}")
+    return cache.shape[2] * KV4_BLOCK
+
+
+def _same_device(who: str, *tensors) -> None:
+    """All on the current device: the launch goes to its current stream."""
+    here = -1
+    for t in tensors:
+        if t is None:
+            continue
+        index = t.get_device()
+        if index < 0:
+            raise KernelError(f"{who}: every tensor must be a CUDA tensor; cuinfer_b200 has no CPU path")
+        if here < 0:
+            here = torch.cuda.current_device()
+        if index != here:
+            raise KernelError(f"{who}: every tensor must be on the current device (cuda:{here}), got cuda:{index}")
+
+
+def qk_norm_rope_kv4_write(qkv: torch.Tensor, positions: torch.Tensor, slot_mapping: torch.Tensor, q_weight: torch.Tensor | None,
+                           k_weight: torch.Tensor | None, eps: float, rope_table: torch.Tensor | None, rotary_dim: int,
+                           cache: torch.Tensor, num_q_heads: int, num_kv_heads: int, head_dim: int, *,
+                           q_out: torch.Tensor | None = None) -> None:
+    """``qk_norm_rope_kv_write`` for a cache held in 4 bits (``kv4_cache_shape``): per-head RMSNorm (if weights are given) and rotary
+    encoding (if a table is given) of the query and key heads of the packed ``qkv`` rows; keys and values are quantised in
+    groups of 32 values and appended to the slots ``slot_mapping`` (-1: none; no slot twice in a call).  The queries go to
+    ``q_out`` [T, nq*d], or replace those of ``qkv`` where none is given; keys and values of ``qkv`` stay as they are."""
+    who = "qk_norm_rope_kv4_write"
+    if qkv.dim() != 2 or qkv.stride(1) != 1:
+        raise KernelError(f"{who}: qkv must be [T, (nq + 2 nkv) * d] with dense rows")
+    T = qkv.shape[0]
+    if qkv.shape[1] < (num_q_heads + 2 * num_kv_heads) * head_dim:
+        raise KernelError(f"{who}: qkv rows of {qkv.shape[1]} values do not hold {num_q_heads} + 2 x {num_kv_heads} heads of {head_dim}")
+    page_size = _kv4_cache(cache, num_kv_heads, head_dim, who)
+    if q_out is None:
+        q_out = qkv
+    elif q_out.shape != (T, num_q_heads * head_dim) or q_out.dtype != qkv.dtype or q_out.stride(1) != 1:
+        raise KernelError(f"{who}: q_out must be {qkv.dtype} [{T}, {num_q_heads * head_dim}] with dense rows")
+    if positions.numel() < T or slot_mapping.numel() < T:
+        raise KernelError(f"{who}: a position and a slot for each of the {T} tokens")
+    has_norm = q_weight is not None
+    if (k_weight is not None) != has_norm or (has_norm and q_weight.dtype != k_weight.dtype):
+        raise KernelError(f"{who}: q and k norm weights must both be given, in one dtype")
+    if has_norm and (q_weight.numel() != head_dim or k_weight.numel() != head_dim):
+        raise KernelError(f"{who}: norm weights must have {head_dim} elements")
+    if rope_table is not None and (rope_table.dim() != 3 or rope_table.shape[1] * 2 != rotary_dim or rope_table.shape[2] != 2):
+        raise KernelError(f"{who}: rope table must be [positions, {rotary_dim // 2}, 2], got {list(rope_table.shape)}")
+    _same_device(who, qkv, cache, q_out, positions, slot_mapping, q_weight, k_weight, rope_table)
+    rc = library().cib_qk_norm_rope_kv4_write(
+        _cuda(qkv, "qkv", contiguous=False), _code(qkv, "qkv"), _row_stride(qkv), _cuda(q_out, "q_out", contiguous=False), _row_stride(q_out),
+        _cuda(positions, "positions", torch.int32), _cuda(slot_mapping, "slot_mapping", torch.int32),
+        _cuda(q_weight, "q_weight") if has_norm else None, _cuda(k_weight, "k_weight") if has_norm else None,
+        _code(q_weight, "q_weight") if has_norm else 0, 1 if has_norm else 0, float(eps),
+        _cuda(rope_table, "rope_table", torch.float32) if rope_table is not None else None,
+        rotary_dim if rope_table is not None else 0, rope_table.shape[0] if rope_table is not None else 0,
+        _cuda(cache, "cache"), cache.shape[0], page_size, T, num_q_heads, num_kv_heads, head_dim, 1 if use_pdl else 0, _stream())
+    _check(rc, who)
+    _count()
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements from a row to the next (of a single row: its length, whatever torch calls its stride)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def kv4_read(cache: torch.Tensor, slots: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, num_kv_heads: int, head_dim: int) -> None:
+    """keys[t], values[t] [nkv * d] = what the cache held in 4 bits holds at ``slots[t]``, as float32 or bfloat16 (in both exactly what
+    the attention multiplies).  Rows of a slot that is none (-1) are left as they are."""
+    who = "kv4_read"
+    page_size = _kv4_cache(cache, num_kv_heads, head_dim, who)
+    T, width = slots.numel(), num_kv_heads * head_dim
+    for name, t in (("keys", keys), ("values", values)):
+        if t.shape != (T, width) or t.dtype != keys.dtype or t.stride(1) != 1:
+            raise KernelError(f"{who}: {name} must be {keys.dtype} [{T}, {width}] with dense rows")
+    _same_device(who, cache, slots, keys, values)
+    rc = library().cib_kv4_read(_cuda(cache, "cache"), cache.shape[0], page_size, _cuda(slots, "slots", torch.int32),
+                                _cuda(keys, "keys", contiguous=False), _row_stride(keys), _cuda(values, "values", contiguous=False),
+                                _row_stride(values), _code(keys, "keys"), T, num_kv_heads, head_dim, 1 if use_pdl else 0, _stream())
+    _check(rc, who)
+    _count()
+
+
+def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, query_start_loc: torch.Tensor,
+                        seq_lens: torch.Tensor, query_lens_host, num_q_heads: int, num_kv_heads: int, head_dim: int, scale: float,
+                        window: int = 0, *, max_seq_len: int) -> None:
+    """Causal attention of the packed query rows ``q[:, :nq*d]`` over a paged cache held in 4 bits (``kv4_cache_shape``); out[T, nq*d].
+    Request r brings the rows ``query_start_loc[r]`` to ``query_start_loc[r + 1]``, the last tokens of its ``seq_lens[r]``; its pages
+    are row r of ``block_table`` (a page that is none, -1: its keys are left out).  ``window`` > 0: a query sees the last so many
+    keys.  Rows that see no key are zero; rows behind the last request are left as they are.  ``query_lens_host``: how many rows
+    each request brings (host ints, or an upper bound as ``StepContext.query_lens_for_launch`` gives); ``max_seq_len``: no request
+    has more keys.  Both shape the launch only.  float32 or bfloat16."""
+    who = "paged_attention_kv4"
+    T = q.shape[0]
+    page_size = _kv4_cache(cache, num_kv_heads, head_dim, who)
+    if num_q_heads <= 0 or num_q_heads % num_kv_heads:
+        raise KernelError(f"{who}: {num_q_heads} query heads do not share {num_kv_heads} key heads")
+    width = num_q_heads * head_dim
+    if q.dim() != 2 or q.stride(1) != 1 or q.shape[1] < width or out.shape != (T, width) or out.stride(1) != 1 or out.dtype != q.dtype:
+        raise KernelError(f"{who}: q must hold rows of {width} values, dense, and out be {q.dtype} [{T}, {width}]")
+    R = seq_lens.numel()
+    if query_start_loc.numel() != R + 1 or block_table.dim() != 2 or block_table.shape[0] < R or len(query_lens_host) != R:
+        raise KernelError(f"{who}: query_start_loc must be [R + 1], block_table [R, pages] and query_lens_host name R requests for the R = {R} of seq_lens")
+    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+        raise KernelError(f"{who}: block_table rows must be dense")
+    if window < 0 or max_seq_len < 0:
+        raise KernelError(f"{who}: window and max_seq_len must not be negative")
+    _same_device(who, q, out, cache, block_table, query_start_loc, seq_lens)
+    if T == 0 or R == 0:
+        return
+    rc = library().cib_attention_kv4_generic(
+        _cuda(q, "q", contiguous=False), _code(q, "q"), _row_stride(q), _cuda(out, "out", contiguous=False), _row_stride(out),
+        _cuda(cache, "cache"), cache.shape[0], page_size, _cuda(block_table, "block_table", torch.int32, contiguous=False),
+        _row_stride(block_table), _cuda(query_start_loc, "query_start_loc", torch.int32), _cuda(seq_lens, "seq_lens", torch.int32), T, R,
+        max_seq_len, 1, num_q_heads, num_kv_heads, head_dim, float(scale), int(window), 1 if use_pdl else 0, _stream())
+    _check(rc, who)
     _count()
 
 

@@ -7,6 +7,9 @@ write of keys and values to the request's pages; attention of every query over i
 0..position read back from the pages (csrc/ops/paged_attention.cu:198-276), consecutive query heads
 sharing a key/value head; output projection.
 
+A cache held in 4 bits (``kv.cache`` of bytes) is written and read by kernels of its own: what is attended over is always what
+the cache holds, the step's own tokens included.
+
 Spec: ``PartSpec("attention", num_heads, num_kv_heads, head_dim, qk_norm, qk_norm_eps, scale, window,
 position=PartSpec(...))``; ``scale`` None means ``head_dim ** -0.5``; ``window`` None means all keys.
 """
@@ -19,7 +22,7 @@ import torch
 from .. import kernels
 from . import attention_dispatch
 from .base import Mixer
-from .context import StepContext
+from .context import PagedKV, StepContext
 from .linear import Linear
 from .registry import MIXERS, POSITION_ENCODINGS
 from .spec import PagedCacheNeed, PartSpec, TensorSpec
@@ -85,6 +88,9 @@ class PagedAttention(Mixer):
     def cache_need(self) -> Optional[PagedCacheNeed]:
         return PagedCacheNeed(self.num_kv_heads, self.head_dim, self.window or None)
 
+    def takes_kv4(self, page_size: int) -> bool:
+        return kernels.kv4_supports(self.head_dim, page_size)
+
     @property
     def capturable(self) -> bool:
         return self.position.capturable
@@ -107,11 +113,19 @@ class PagedAttention(Mixer):
     def _attend(self, x: torch.Tensor, ctx: StepContext, run: int) -> torch.Tensor:
         kv = ctx.paged_kv(run)
         qkv = self.qkv.forward(x)
+        if kv.writes and kv.cache.dtype == torch.uint8:
+            kernels.qk_norm_rope_kv4_write(
+                qkv, ctx.positions, kv.group.slot_mapping, self.q_norm_weight, self.k_norm_weight, self.qk_norm_eps,
+                self.position.table(), self.position.rotary_dim, kv.cache, self.num_heads, self.num_kv_heads, self.head_dim)
+            return self._over_cache(qkv, kv, ctx)
         kernels.qk_norm_rope_kv_write(
             qkv, ctx.positions, kv.group.slot_mapping if kv.writes else None,
             self.q_norm_weight, self.k_norm_weight, self.qk_norm_eps,
             self.position.table(), self.position.rotary_dim,
             kv.cache if kv.writes else None, self.num_heads, self.num_kv_heads, self.head_dim)
+        return self._over_cache(qkv, kv, ctx)
+
+    def _over_cache(self, qkv: torch.Tensor, kv: PagedKV, ctx: StepContext) -> torch.Tensor:
         out = torch.empty((qkv.shape[0], self.q_size), dtype=qkv.dtype, device=qkv.device)
         attention_dispatch.paged_attention(qkv, out, kv, ctx, self.num_heads, self.num_kv_heads, self.head_dim,
                                            self.scale, self.window, warm=self.o.weight)

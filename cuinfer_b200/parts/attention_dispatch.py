@@ -1,7 +1,7 @@
 """Choice of the paged-attention kernel for a step (keys and values per head; attention over cached latents: see
 ``latent_attention`` at the end).
 
-float32 always runs the all-sizes kernel.  bfloat16: a step of single decoded tokens runs the split-KV kernel (its
+A cache held in 4 bits: ``kernels.paged_attention_kv4``, which chooses by itself.  Else: float32 always runs the all-sizes kernel.  bfloat16: a step of single decoded tokens runs the split-KV kernel (its
 TMA path where the cache layout allows and a CTA streams at least ``kernels.DECODE_TMA_MIN_KEYS`` keys, else its
 cp.async path); any
 other step runs the tcgen05 kernel (head size 128, heads per kv head dividing 128) or the mma.sync kernel (head
@@ -57,6 +57,10 @@ def paged_attention(qkv: torch.Tensor, out: torch.Tensor, kv: PagedKV, ctx: Step
                     num_kv_heads: int, head_dim: int, scale: float, window: int, warm: torch.Tensor | None = None) -> None:
     """``warm``: what the step reads right after the attention (the output projection's weight); the decode kernel
     asks for it to be fetched into the L2 when its stream of keys ends."""
+    if kv.cache.dtype == torch.uint8:
+        kernels.paged_attention_kv4(qkv, out, kv.cache, kv.group.block_table, ctx.query_start_loc, ctx.seq_lens, ctx.query_lens_for_launch(),
+                                    num_heads, num_kv_heads, head_dim, scale, window, max_seq_len=max(1, ctx.max_seq_len))
+        return
     if (qkv.dtype == torch.bfloat16 and ctx.decode_only
             and kernels.paged_attention_decode_supports(head_dim, num_heads, num_kv_heads)):
         _decode(qkv, out, kv, ctx, num_heads, num_kv_heads, head_dim, scale, window, warm)

@@ -286,6 +286,10 @@ class Mixer(Part):
     def state_need(self) -> Optional[StateNeed]:
         return None
 
+    def takes_kv4(self, page_size: int) -> bool:
+        """Whether the mixer writes and reads a paged cache that is held in 4 bits."""
+        return False
+
     def forward(self, x: torch.Tensor, ctx: StepContext, run: int) -> torch.Tensor:
         raise NotImplementedError
 

@@ -25,7 +25,8 @@ class GroupView:
 
 @dataclass
 class PagedKV:
-    """The cache of one run of a layer: ``cache[page, 0|1, kv_head, slot, d]`` with its group's addressing.
+    """The cache of one run of a layer: ``cache[page, 0|1, kv_head, slot, d]`` with its group's addressing, or bytes
+    ``cache[page, kv_head, block, 18 d]`` where it is held in 4 bits.
 
     ``writes`` is False when the run reads the cache that an earlier run filled.
     """
