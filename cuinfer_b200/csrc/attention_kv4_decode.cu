@@ -1,0 +1,419 @@
+// Attention of single tokens over the cache that is held in 4 bits (kv4.cuh): bfloat16, head size 64, 128 or 256.
+//
+// Decode is a stream of the cache through the SMs: 9/8 D bytes a token and kv head.  The 16-token blocks of a (request, kv head) are
+// split over `splits` CTAs and inside a CTA over four warps; a warp copies two blocks at a time into a private ring
+// of shared memory (a block is one contiguous piece: one `cp.async.bulk` each, counted on an mbarrier) and multiplies them with up to
+// eight query heads by mma.m16n8k16 with the quantised operand as A (16 keys, or 16 value columns) and the heads as the 8 columns:
+//
+//   scores   S^T[key, head] = sum over groups g of step[key, g] * (sum of (128 + code) q - 128 sum of q) - sum over g of step zero sum_g(q)
+//            A code c becomes the bfloat16 128 + c by one shift and one three-input logic operation for two codes; the accumulator
+//            starts at -128 sum_g(q), and the zero points of all groups are one more MMA with step * zero (exact: four bits
+//            times four) against the sums of q, which are split into bfloat16 parts.  All operands are exact.
+//   values   O^T[column, head] += sum over keys of (code - zero) * (p step),  p = 2^(s - m): only p * step is rounded, once.
+//            The weights come out of the scores with keys as rows and go in with keys as the summed index: one 8 x 8 transposition in
+//            registers (movmatrix) for 8 keys.
+//
+// A running maximum and sum per head in base 2, in 32 bits; warps are merged in shared memory, CTAs by a second kernel from partial results in
+// scratch memory that the caller brings: [(request, head)][split][D] and [..][2] (nothing global is counted or kept, so any
+// number of launches may run at once).
+#include "kv4.cuh"
+#include "mma_utils.cuh"
+#include "tcgen05_utils.cuh"
+
+namespace cib {
+namespace kv4 {
+
+constexpr int kDecWarps = 4;
+constexpr int kDecStages = 3;
+constexpr int kDecHeads = 8;         // query heads of a CTA: the columns of an MMA
+
+template <int D>
+constexpr int stage_bytes() { return 2 * block_bytes(D); }
+template <int D>
+constexpr int ring_bytes() { return kDecWarps * kDecStages * stage_bytes<D>(); }
+
+// the blocks [first, first + count) of a request that its last token sees, and how many of them a CTA takes
+struct Span {
+    int first, count, chunk;
+};
+__device__ __forceinline__ Span span_of(int seq_len, int window, int splits) {
+    Span s;
+    const int lo = window > 0 ? max(0, seq_len - window) : 0;
+    s.first = lo / kBlock;
+    s.count = max(0, (seq_len + kBlock - 1) / kBlock - s.first);
+    constexpr int unit = 2 * kDecWarps;                          // two blocks for every warp
+    s.chunk = max(1, (s.count + splits * unit - 1) / (splits * unit)) * unit;
+    return s;
+}
+
+template <int N>
+struct alignas(N * 4) Words {
+    uint32_t w[N];
+};
+// bfloat16 pairs of codes i of both halves of a word, plus 128
+__device__ __forceinline__ uint32_t pair128(uint32_t w, int i) { return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u; }
+__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+    return r;
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(tc_smem_u32(dst)), "l"(src), "r"(bytes), "r"(tc_smem_u32(bar)) : "memory");
+}
+
+template <int D>
+__global__ void __launch_bounds__(kDecWarps * 32, D > 128 ? 2 : 4)
+attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* __restrict__ out, int out_stride,
+                        const unsigned char* __restrict__ cache, int num_pages, int page_size, const int* __restrict__ block_table, int table_stride,
+                        const int* __restrict__ query_start_loc, const int* __restrict__ seq_lens, int nq, int nkv, float scale_log2, int window,
+                        int splits, float* __restrict__ part_o, float* __restrict__ part_ml, int* __restrict__ error_flag) {
+    constexpr int NG = D / kGroup;
+    constexpr int kBytes = block_bytes(D);
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ uint64_t s_full[kDecWarps * kDecStages];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, row = lane >> 2;
+    const int split = blockIdx.x, r = blockIdx.z;
+    const int g = nq / nkv, head_blocks = (g + kDecHeads - 1) / kDecHeads;
+    const int kvh = blockIdx.y / head_blocks, hb = blockIdx.y - kvh * head_blocks;
+    const int head0 = kvh * g + hb * kDecHeads, nh = min(kDecHeads, g - hb * kDecHeads);
+
+    if (lane < kDecStages) mbar_init(&s_full[warp * kDecStages + lane], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    const int token = query_start_loc[r];
+    const bool mine = query_start_loc[r + 1] - token == 1;
+    const int seq_len = seq_lens[r];
+    griddep_wait();          // queries and this step's keys and values come from the kernel before
+    griddep_launch();
+    if (!mine) return;
+    const Span span = span_of(seq_len, window, splits);
+    if (split != 0 && split * span.chunk >= span.count) return;
+    const bool alone = span.chunk >= span.count;
+    const int begin = span.first + split * span.chunk, end = min(span.first + span.count, begin + span.chunk);
+    const int lo = window > 0 ? max(0, seq_len - window) : 0;
+    const int* table = block_table + (size_t)r * table_stride;
+    const int per_page = page_size / kBlock;
+
+    // this warp's pairs of blocks: begin + 2 (i * warps + warp), i = 0 .. mine_pairs - 1
+    const int pairs = (end - begin + 1) / 2;
+    const int count = pairs > warp ? (pairs - warp + kDecWarps - 1) / kDecWarps : 0;
+    unsigned char* ring = smem + warp * kDecStages * stage_bytes<D>();
+    uint64_t* full = s_full + warp * kDecStages;
+    // lanes 2 j and 2 j + 1 look up the blocks of pair 16 n + j, a batch of 16 pairs ahead of its use
+    auto lookup = [&](int batch) {
+        const int i = batch * 16 + (lane >> 1);
+        const int b = begin + 2 * (i * kDecWarps + warp) + (lane & 1);
+        if (i >= count || b >= end) return -1;
+        const int index = b / per_page;
+        if (index >= table_stride) return -1;
+        const int page = table[index];
+        return page >= 0 && page < num_pages ? (page * nkv + kvh) * per_page + (b - index * per_page) : -1;
+    };
+    int ids = lookup(0), ids_next = lookup(1);
+    uint32_t present = 0;            // two bits a ring stage: which of its blocks the table names
+    auto request = [&](int i) {
+        if (i != 0 && (i & 15) == 0) {
+            ids = ids_next;
+            ids_next = lookup((i >> 4) + 1);
+        }
+        const int s = i % kDecStages;
+        const uint32_t here = (__ballot_sync(0xffffffffu, ids >= 0) >> (2 * (i & 15))) & 3u;
+        present = (present & ~(3u << (2 * s))) | (here << (2 * s));
+        if (lane == 0) mbar_expect_tx(&full[s], __popc(here) * kBytes);
+        __syncwarp();
+        if ((lane >> 1) == (i & 15) && ids >= 0)
+            bulk_load(ring + s * stage_bytes<D>() + (lane & 1) * kBytes, cache + (size_t)ids * kBytes, kBytes, &full[s]);
+    };
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kDecStages - 1; ++i)
+        if (i < count) request(i);
+
+    // ---- queries: the B operand, head = column `row`; a lane has values 32 g + 8 quad .. + 7 of every group ----
+    uint32_t qf[NG][4];
+    {
+        const __nv_bfloat16* qp = q + (size_t)token * q_stride + (size_t)(head0 + row) * D + 8 * quad;
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (row < nh) v = *reinterpret_cast<const uint4*>(qp + k * kGroup);
+            qf[k][0] = v.x, qf[k][1] = v.y, qf[k][2] = v.z, qf[k][3] = v.w;
+        }
+    }
+    // -128 sum_g(q) of heads 2 quad and 2 quad + 1; minus the sums in bfloat16 parts as the B operand of the zero points
+    float start[NG][2];
+    uint32_t sums0 = 0, sums1 = 0;
+    constexpr int kPairs = NG / 2;
+    const int my_pair = quad % kPairs;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        mma16816(acc, 0xc300c300u, 0xc300c300u, 0xc300c300u, 0xc300c300u, qf[k][0], qf[k][1]);
+        mma16816(acc, 0xc300c300u, 0xc300c300u, 0xc300c300u, 0xc300c300u, qf[k][2], qf[k][3]);
+        start[k][0] = acc[0], start[k][1] = acc[1];
+        float sum = 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sum += __uint_as_float(qf[k][u] << 16) + __uint_as_float(qf[k][u] & 0xffff0000u);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        // parts of 8 bits; the summed index of the MMA runs over (part, group pair): quads hold part quad / kPairs, then the next ones
+        float rest = -sum;
+        uint32_t part[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const __nv_bfloat16 h = __float2bfloat16_rn(rest);
+            part[u] = __bfloat16_as_ushort(h);
+            rest -= __bfloat162float(h);
+        }
+        constexpr int kFirst = 4 / kPairs;                      // parts in the first half of the index
+        if ((k >> 1) == my_pair) {
+            const int p0 = quad / kPairs, p1 = kFirst + p0;
+            const uint32_t a = p0 == 0 ? part[0] : p0 == 1 ? part[1] : p0 == 2 ? part[2] : part[3];
+            const uint32_t b = p1 == 1 ? part[1] : p1 == 2 ? part[2] : p1 == 3 ? part[3] : 0u;
+            sums0 |= a << (16 * (k & 1));
+            sums1 |= b << (16 * (k & 1));
+        }
+    }
+
+    float o[2 * NG][4];
+#pragma unroll
+    for (int i = 0; i < 2 * NG; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (int i = 0; i < count; ++i) {
+        const int st = i % kDecStages;
+        const bool landed = __all_sync(0xffffffffu, mbar_wait(&full[st], (uint32_t)((i / kDecStages) & 1)));
+        if (!landed) {
+            if (lane == 0) atomicExch(error_flag, 41);
+            break;
+        }
+        // the stage that pair i - 1 was read from is refilled: every lane has finished reading it
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (i + kDecStages - 1 < count) request(i + kDecStages - 1);
+        const unsigned char* stage = ring + st * stage_bytes<D>();
+        const int block0 = begin + 2 * (i * kDecWarps + warp);
+        const uint32_t here = (present >> (2 * st)) & 3u;
+        const bool whole = here == 3u && block0 * kBlock >= lo && (block0 + 2) * kBlock <= seq_len;
+
+        // ---- scores of 32 keys ----
+        float s[2][4];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const unsigned char* block = stage + b * kBytes;
+            const Words<NG> c0 = reinterpret_cast<const Words<NG>*>(block)[lane], c1 = reinterpret_cast<const Words<NG>*>(block)[32 + lane];
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(block + key_words_at(D));
+            const Words<kPairs> w0 = reinterpret_cast<const Words<kPairs>*>(words)[row], w1 = reinterpret_cast<const Words<kPairs>*>(words)[row + 8];
+            {
+                const uint32_t a = words[row * kPairs + my_pair], c = words[(row + 8) * kPairs + my_pair];
+                const uint32_t za = mul_bf16x2(sub_bf16x2((a & 0x000f000fu) | 0x43004300u, 0x43004300u), a & 0xfff0fff0u);
+                const uint32_t zc = mul_bf16x2(sub_bf16x2((c & 0x000f000fu) | 0x43004300u, 0x43004300u), c & 0xfff0fff0u);
+                s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
+                mma16816(s[b], za, zc, za, zc, sums0, sums1);
+            }
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+                float acc[4] = {start[k][0], start[k][1], start[k][0], start[k][1]};
+                mma16816(acc, pair128(c0.w[k], 0), pair128(c1.w[k], 0), pair128(c0.w[k], 1), pair128(c1.w[k], 1), qf[k][0], qf[k][1]);
+                mma16816(acc, pair128(c0.w[k], 2), pair128(c1.w[k], 2), pair128(c0.w[k], 3), pair128(c1.w[k], 3), qf[k][2], qf[k][3]);
+                const uint32_t a = w0.w[k >> 1], c = w1.w[k >> 1];
+                const float sa = __uint_as_float((k & 1 ? a : a << 16) & 0xfff00000u), sc = __uint_as_float((k & 1 ? c : c << 16) & 0xfff00000u);
+                s[b][0] = fmaf(sa, acc[0], s[b][0]);
+                s[b][1] = fmaf(sa, acc[1], s[b][1]);
+                s[b][2] = fmaf(sc, acc[2], s[b][2]);
+                s[b][3] = fmaf(sc, acc[3], s[b][3]);
+            }
+        }
+        bool seen[2][2] = {{true, true}, {true, true}};
+        if (!whole) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int key = (block0 + b) * kBlock + row + 8 * h;
+                    seen[b][h] = ((here >> b) & 1u) && key >= lo && key < seq_len;
+                    if (!seen[b][h]) s[b][2 * h] = s[b][2 * h + 1] = -INFINITY;
+                }
+        }
+        // ---- running maximum; heads 2 quad (e = 0) and 2 quad + 1 ----
+        float top[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float x = fmaxf(fmaxf(s[0][e], s[0][2 + e]), fmaxf(s[1][e], s[1][2 + e])) ;
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            top[e] = fmaxf(m[e], x * scale_log2);
+        }
+        if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+            float corr[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                corr[e] = m[e] == -INFINITY ? 0.f : ex2(m[e] - top[e]);
+                m[e] = top[e];
+                l[e] *= corr[e];
+            }
+#pragma unroll
+            for (int t = 0; t < 2 * NG; ++t) o[t][0] *= corr[0], o[t][1] *= corr[1], o[t][2] *= corr[0], o[t][3] *= corr[1];
+        }
+        const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+        // ---- weights and values ----
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                p[e] = ex2(fmaf(s[b][e], scale_log2, -base[e & 1]));
+                l[e & 1] += p[e];
+            }
+            const unsigned char* block = stage + b * kBytes;
+            const Words<NG>* words = reinterpret_cast<const Words<NG>*>(block + value_words_at(D));
+            const Words<NG> a0 = words[row >> 1], a1 = words[4 + (row >> 1)], z0 = words[quad], z1 = words[4 + quad];
+            const Words<NG>* codes = reinterpret_cast<const Words<NG>*>(block + value_codes_at(D));
+            const Words<NG> v0 = codes[lane], v1 = codes[32 + lane];
+            const int up = row & 1 ? 0 : 16;
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+                float sa = __uint_as_float((a0.w[k] << up) & 0xfff00000u), sc = __uint_as_float((a1.w[k] << up) & 0xfff00000u);
+                if (!whole) {                                   // what lies where no token has been written may be anything
+                    sa = seen[b][0] ? sa : 0.f;
+                    sc = seen[b][1] ? sc : 0.f;
+                }
+                const uint32_t b0 = transpose8(pack_bf16(p[0] * sa, p[1] * sa)), b1 = transpose8(pack_bf16(p[2] * sc, p[3] * sc));
+                const uint32_t za = (z0.w[k] & 0x000f000fu) | 0x43004300u, zc = (z1.w[k] & 0x000f000fu) | 0x43004300u;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    mma16816(o[2 * k + t], sub_bf16x2(pair128(v0.w[k], 2 * t), za), sub_bf16x2(pair128(v0.w[k], 2 * t + 1), za),
+                             sub_bf16x2(pair128(v1.w[k], 2 * t), zc), sub_bf16x2(pair128(v1.w[k], 2 * t + 1), zc), b0, b1);
+            }
+        }
+    }
+    __syncthreads();     // all rings have been read
+    // ---- merge the warps: [warp][head][D] values, [warp][head] maxima and sums ----
+    float* sm_o = reinterpret_cast<float*>(smem);
+    float* sm_m = sm_o + kDecWarps * kDecHeads * D;
+    float* sm_l = sm_m + kDecWarps * kDecHeads;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        float x = l[e];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        const int head = 2 * quad + e;
+        if (row == 0) sm_m[warp * kDecHeads + head] = m[e], sm_l[warp * kDecHeads + head] = x;
+        float4* dst = reinterpret_cast<float4*>(sm_o + (size_t)(warp * kDecHeads + head) * D) + row;
+#pragma unroll
+        for (int k = 0; k < NG; ++k) dst[k * 8] = make_float4(o[2 * k][e], o[2 * k][2 + e], o[2 * k + 1][e], o[2 * k + 1][2 + e]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < nh * D; i += kDecWarps * 32) {
+        const int h = i / D, x = i - h * D;
+        float M = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll
+        for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, sm_m[w * kDecHeads + h]);
+#pragma unroll
+        for (int w = 0; w < kDecWarps; ++w) {
+            const float f = sm_m[w * kDecHeads + h] == -INFINITY ? 0.f : ex2(sm_m[w * kDecHeads + h] - M);
+            L += sm_l[w * kDecHeads + h] * f;
+            O += sm_o[(size_t)(w * kDecHeads + h) * D + x] * f;
+        }
+        if (alone) {
+            out[(size_t)token * out_stride + (size_t)(head0 + h) * D + x] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L);
+        } else {
+            const size_t at = ((size_t)r * nq + head0 + h) * splits + split;
+            part_o[at * D + x] = O;
+            if (x == 0) part_ml[at * 2] = M, part_ml[at * 2 + 1] = L;
+        }
+    }
+}
+
+// A CTA per (request, query head), a thread per value.
+template <int D>
+__global__ void __launch_bounds__(D)
+attention_decode_merge_kernel(__nv_bfloat16* __restrict__ out, int out_stride, const int* __restrict__ query_start_loc, const int* __restrict__ seq_lens,
+                              int nq, int window, int splits, const float* __restrict__ part_o, const float* __restrict__ part_ml) {
+    const int head = blockIdx.x, r = blockIdx.y, x = threadIdx.x;
+    const int token = query_start_loc[r];
+    const bool mine = query_start_loc[r + 1] - token == 1;
+    const Span span = span_of(seq_lens[r], window, splits);
+    griddep_wait();
+    griddep_launch();
+    if (!mine || span.chunk >= span.count) return;
+    const int active = (span.count + span.chunk - 1) / span.chunk;
+    const size_t at = ((size_t)r * nq + head) * splits;
+    float M = -INFINITY, L = 0.f, O = 0.f;
+    for (int s = 0; s < active; ++s) M = fmaxf(M, part_ml[(at + s) * 2]);
+#pragma unroll 8
+    for (int s = 0; s < active; ++s) {
+        const float m = part_ml[(at + s) * 2], f = m == -INFINITY ? 0.f : ex2(m - M);
+        L += part_ml[(at + s) * 2 + 1] * f;
+        O += part_o[(at + s) * D + x] * f;
+    }
+    out[(size_t)token * out_stride + (size_t)head * D + x] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L);
+}
+
+}  // namespace kv4
+}  // namespace cib
+
+using namespace cib;
+
+extern "C" int cib_attention_kv4_decode_supports(int d, int page_size) {
+    return kv4::sizes_ok(d, page_size) && (d == 64 || d == 128 || d == 256);
+}
+
+// Computes the rows of the requests that bring one token; the others' are left as they are.  scratch: splits * requests * nq * (d + 2)
+// floats where splits > 1.
+extern "C" int cib_attention_kv4_decode(const void* q, int q_stride, void* out, int out_stride, const void* cache, int num_pages, int page_size,
+                                        const int* block_table, int table_stride, const int* query_start_loc, const int* seq_lens, int num_requests, int nq,
+                                        int nkv, int d, float scale, int window, int splits, float* scratch, int* error_flag, int use_pdl, cudaStream_t stream) {
+    CIB_REQUIRE(cib_attention_kv4_decode_supports(d, page_size), "attention_kv4_decode: head size %d (64, 128 or 256), page size %d (a multiple of 16) are not taken", d, page_size);
+    CIB_REQUIRE(num_requests >= 0 && num_requests <= 65535 && nq > 0 && nkv > 0 && nq % nkv == 0, "attention_kv4_decode: bad sizes R=%d nq=%d nkv=%d", num_requests, nq, nkv);
+    CIB_REQUIRE(splits >= 1 && (splits == 1 || scratch != nullptr), "attention_kv4_decode: scratch missing");
+    CIB_REQUIRE(num_pages > 0 && table_stride > 0 && cache != nullptr && ((uintptr_t)cache % 16) == 0, "attention_kv4_decode: bad cache geometry");
+    CIB_REQUIRE((long long)num_pages * nkv * (page_size / kv4::kBlock) < (1ll << 31), "attention_kv4_decode: more than 2^31 blocks");
+    CIB_REQUIRE(q_stride % 8 == 0 && ((uintptr_t)q % 16) == 0, "attention_kv4_decode: query rows must be 16-byte aligned");
+    CIB_REQUIRE(window >= 0 && error_flag != nullptr, "attention_kv4_decode: window must be >= 0, error flag given");
+    const int g = nq / nkv, head_blocks = (g + kv4::kDecHeads - 1) / kv4::kDecHeads;
+    CIB_REQUIRE((long long)nkv * head_blocks <= 65535, "attention_kv4_decode: too many heads");
+    if (num_requests == 0) return 0;
+    const float scale_log2 = scale * 1.4426950408889634f;
+    float* part_ml = scratch == nullptr ? nullptr : scratch + (size_t)num_requests * nq * splits * d;
+    const dim3 grid(splits, nkv * head_blocks, num_requests);
+#define CIB_KV4_DECODE(DV)                                                                                                                           \
+    if (d == DV) {                                                                                                                                   \
+        static SmemLimit limit;                                                                                                                      \
+        if (int rc = raise_smem_limit(limit, kv4::attention_decode_kernel<DV>, kv4::ring_bytes<DV>(), "attention_kv4_decode")) return rc;            \
+        cudaError_t e = launch_pdl(kv4::attention_decode_kernel<DV>, grid, dim3(kv4::kDecWarps * 32), (size_t)kv4::ring_bytes<DV>(), stream,         \
+                                   use_pdl != 0, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, (const unsigned char*)cache,     \
+                                   num_pages, page_size, block_table, table_stride, query_start_loc, seq_lens, nq, nkv, scale_log2, window, splits,   \
+                                   scratch, part_ml, error_flag);                                                                                    \
+        if (e == cudaSuccess && splits > 1)                                                                                                          \
+            e = launch_pdl(kv4::attention_decode_merge_kernel<DV>, dim3(nq, num_requests), dim3(DV), 0, stream, use_pdl != 0, (__nv_bfloat16*)out,   \
+                           out_stride, query_start_loc, seq_lens, nq, window, splits, scratch, part_ml);                                             \
+        CIB_REQUIRE(e == cudaSuccess, "attention_kv4_decode: launch failed: %s", cudaGetErrorString(e));                                             \
+        return 0;                                                                                                                                    \
+    }
+    CIB_KV4_DECODE(64)
+    CIB_KV4_DECODE(128)
+    CIB_KV4_DECODE(256)
+#undef CIB_KV4_DECODE
+    return -1;
+}

@@ -122,6 +122,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "cib_qk_norm_rope_kv4_write": [_P, _I, _I, _P, _I, _P, _P, _P, _P, _I, _I, _F, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P],
         "cib_kv4_read": [_P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
         "cib_attention_kv4_generic": [_P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
+        "cib_attention_kv4_decode": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _F, _I, _I, _P, _P, _I, _P],
         "cib_gemm_skinny": [_P, _I, _I, _I, _P, _I, _P, _P, _I, _P, _I, _F, _P, _P, _I, _I, _I, _I, _I, _P, ctypes.c_longlong, _P, _I, _P, _P, _P],
         "cib_gemm_tcgen05": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P, _I, _F, _P, _P, _I, _P, _P, _P],
         "cib_gemm_wstream": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _P, _I, _F, _P, _P, _I, _P, _P, _I, _P, ctypes.c_longlong, _I, _P, _P],
@@ -152,6 +153,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.cib_latent_attention_mma_tiles.restype = _I
     lib.cib_paged_attention_decode_supports.argtypes = [_I, _I, _I]
     lib.cib_paged_attention_decode_supports.restype = _I
+    lib.cib_attention_kv4_decode_supports.argtypes = [_I, _I]
+    lib.cib_attention_kv4_decode_supports.restype = _I
     lib.cib_gemm_tcgen05_supports.argtypes = [_I, _I, _I]
     lib.cib_gemm_tcgen05_supports.restype = _I
     lib.cib_gemm_tcgen05_stream_cols.argtypes = [_I, _I, _I]
@@ -881,13 +884,37 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
     _same_device(who, q, out, cache, block_table, query_start_loc, seq_lens)
     if T == 0 or R == 0:
         return
-    rc = library().cib_attention_kv4_generic(
-        _cuda(q, "q", contiguous=False), _code(q, "q"), _row_stride(q), _cuda(out, "out", contiguous=False), _row_stride(out),
-        _cuda(cache, "cache"), cache.shape[0], page_size, _cuda(block_table, "block_table", torch.int32, contiguous=False),
-        _row_stride(block_table), _cuda(query_start_loc, "query_start_loc", torch.int32), _cuda(seq_lens, "seq_lens", torch.int32), T, R,
-        max_seq_len, 1, num_q_heads, num_kv_heads, head_dim, float(scale), int(window), 1 if use_pdl else 0, _stream())
+    cache_args = (_cuda(cache, "cache"), cache.shape[0], page_size, _cuda(block_table, "block_table", torch.int32, contiguous=False),
+                  _row_stride(block_table), _cuda(query_start_loc, "query_start_loc", torch.int32), _cuda(seq_lens, "seq_lens", torch.int32))
+    q_args = (_cuda(q, "q", contiguous=False), _row_stride(q))
+    out_args = (_cuda(out, "out", contiguous=False), _row_stride(out))
+    dtype = _code(q, "q")
+    pdl = 1 if use_pdl else 0
+    least_query = 1
+    # Single tokens run on the kernel that splits keys; the lengths are a bound where they name more rows than there are, and any
+    # request may then bring a single token.
+    if (dtype == BF16 and library().cib_attention_kv4_decode_supports(head_dim, page_size) and q_args[1] % 8 == 0 and q_args[0] % 16 == 0
+            and (1 in query_lens_host or sum(query_lens_host) > T)):
+        splits = kv4_decode_splits(R * num_kv_heads * -(-(num_q_heads // num_kv_heads) // 8), min(max_seq_len, window or max_seq_len), head_dim)
+        scratch = torch.empty(splits * R * num_q_heads * (head_dim + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+        rc = library().cib_attention_kv4_decode(*q_args, *out_args, *cache_args, R, num_q_heads, num_kv_heads, head_dim, float(scale), int(window), splits,
+                                                scratch.data_ptr() if scratch is not None else None, _error_flag(q.device).data_ptr(), pdl, _stream())
+        _check(rc, who)
+        note_flagged_launch()
+        _count()
+        if T <= R and max(query_lens_host) <= 1:
+            return
+        least_query = 2
+    rc = library().cib_attention_kv4_generic(q_args[0], dtype, q_args[1], *out_args, *cache_args, T, R, max_seq_len, least_query, num_q_heads, num_kv_heads,
+                                             head_dim, float(scale), int(window), pdl, _stream())
     _check(rc, who)
     _count()
+
+
+def kv4_decode_splits(pairs: int, keys: int, head_dim: int) -> int:
+    """How many CTAs share the keys of a (request, kv head)."""
+    slots = 148 * (2 if head_dim > 128 else 4)
+    return max(1, min(64, -(-keys // 128), slots // pairs))
 
 
 # ---- matrix product ----------------------------------------------------------------------------------
