@@ -5,13 +5,18 @@
 // of shared memory (a block is one contiguous piece: one `cp.async.bulk` each, counted on an mbarrier) and multiplies them with up to
 // eight query heads by mma.m16n8k16 with the quantised operand as A (16 keys, or 16 value columns) and the heads as the 8 columns:
 //
-//   scores   S^T[key, head] = sum over groups g of step[key, g] * (sum of (128 + code) q - 128 sum of q) - sum over g of step zero sum_g(q)
-//            A code c becomes the bfloat16 128 + c by one shift and one three-input logic operation for two codes; the accumulator
-//            starts at -128 sum_g(q), and the zero points of all groups are one more MMA with step * zero (exact: four bits
-//            times four) against the sums of q, which are split into bfloat16 parts.  All operands are exact.
-//   values   O^T[column, head] += sum over keys of (code - zero) * (p step),  p = 2^(s - m): only p * step is rounded, once.
-//            The weights come out of the scores with keys as rows and go in with keys as the summed index: one 8 x 8 transposition in
-//            registers (movmatrix) for 8 keys.
+//   scores   S^T[key, head] = sum over groups g of step[key, g] * (sum of code q) - sum over g of step zero sum_g(q)
+//   values   O^T[column, head] += sum over keys of (code - zero) * (p step),  p = 2^(s - m)
+//
+// What bounds such a kernel is taking the codes apart: the integer pipe does one operation in two cycles of a scheduler.  A bfloat16 whose
+// bits are v < 256 is v 2^-133 (its subnormals and the first normal binade are one linear range), so four bits of a word are an
+// operand as they stand: a code masked out of bits 0-3 is c 2^-133, out of bits 4-7 16 c 2^-133, and one shift by 8 serves
+// the other two: 5 operations for 8 codes, where placing each code under an exponent took 7.  The queries are multiplied by a power of
+// two a head, so that their largest lies in [2^126, 2^127), and by 1/16 against the codes of bits 4-7; the scores take it back.
+// The zero points of all groups are one more MMA with step * zero (four bits times four) against the sums of q, which are split into
+// bfloat16 parts.  All operands of the scores are exact.  For the values one fused multiply-add on the other pipe gives (code - zero) 2^-6,
+// also exact; only p * step is rounded, once.  The weights come out of the scores with keys as rows and go in with keys as the summed
+// index: one 8 x 8 transposition in registers (movmatrix) for 8 keys.
 //
 // A running maximum and sum per head in base 2, in 32 bits; warps are merged in shared memory, CTAs by a second kernel from partial results in
 // scratch memory that the caller brings: [(request, head)][split][D] and [..][2] (nothing global is counted or kept, so any
@@ -50,16 +55,14 @@ template <int N>
 struct alignas(N * 4) Words {
     uint32_t w[N];
 };
-// bfloat16 pairs of codes i of both halves of a word, plus 128
-__device__ __forceinline__ uint32_t pair128(uint32_t w, int i) { return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u; }
-__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
 }
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) { return fma_bf16x2(a, b, 0x80008000u); }     // (+ -0)
+// pairs of bfloat16 constants
+constexpr uint32_t k2p127 = 0x7f007f00u, kMinus2p127 = 0xff00ff00u, k2p123 = 0x7d007d00u;
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
@@ -68,6 +71,11 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the same onto zero
+__device__ __forceinline__ void mma16816_0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ float ex2(float x) {
     float r;
@@ -149,6 +157,7 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
 
     // ---- queries: the B operand, head = column `row`; a lane has values 32 g + 8 quad .. + 7 of every group ----
     uint32_t qf[NG][4];
+    float largest = 0.f;
     {
         const __nv_bfloat16* qp = q + (size_t)token * q_stride + (size_t)(head0 + row) * D + 8 * quad;
 #pragma unroll
@@ -156,26 +165,33 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             uint4 v = make_uint4(0, 0, 0, 0);
             if (row < nh) v = *reinterpret_cast<const uint4*>(qp + k * kGroup);
             qf[k][0] = v.x, qf[k][1] = v.y, qf[k][2] = v.z, qf[k][3] = v.w;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) largest = fmaxf(largest, fmaxf(fabsf(__uint_as_float(qf[k][u] << 16)), fabsf(__uint_as_float(qf[k][u] & 0xffff0000u))));
         }
     }
-    // -128 sum_g(q) of heads 2 quad and 2 quad + 1; minus the sums in bfloat16 parts as the B operand of the zero points
-    float start[NG][2];
+    largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+    largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+    // 2^-e for the head's largest |q| in [2^e, 2^(e + 1)); e = 0 for a head of zeros and one that is not finite
+    const int exponent = largest > 1.1754944e-38f && largest < INFINITY ? (int)(__float_as_uint(largest) >> 23) - 127 : 0;
+    const float down = __uint_as_float((uint32_t)(127 - exponent) << 23), tiny = exponent == 127 ? 5.877472e-39f : down;
+    // minus half the sums of the scaled queries in bfloat16 parts: the B operand of the zero points.  The summed index runs over (part,
+    // group pair): quads hold part quad / kPairs of a pair, then the parts behind those.
     uint32_t sums0 = 0, sums1 = 0;
     constexpr int kPairs = NG / 2;
     const int my_pair = quad % kPairs;
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        mma16816(acc, 0xc300c300u, 0xc300c300u, 0xc300c300u, 0xc300c300u, qf[k][0], qf[k][1]);
-        mma16816(acc, 0xc300c300u, 0xc300c300u, 0xc300c300u, 0xc300c300u, qf[k][2], qf[k][3]);
-        start[k][0] = acc[0], start[k][1] = acc[1];
         float sum = 0.f;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) sum += __uint_as_float(qf[k][u] << 16) + __uint_as_float(qf[k][u] & 0xffff0000u);
+        for (int u = 0; u < 4; ++u) {
+            const float a = __uint_as_float(qf[k][u] << 16) * tiny, c = __uint_as_float(qf[k][u] & 0xffff0000u) * tiny;
+            sum += a + c;
+            const float up = u & 1 ? 5.3169119831396635e+36f : 8.507059173023462e+37f;       // 2^122 against 16 c, 2^126 against c
+            qf[k][u] = pack_bf16(a * up, c * up);
+        }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        // parts of 8 bits; the summed index of the MMA runs over (part, group pair): quads hold part quad / kPairs, then the next ones
-        float rest = -sum;
+        float rest = -0.5f * sum;
         uint32_t part[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -192,6 +208,10 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             sums1 |= b << (16 * (k & 1));
         }
     }
+    // a sum of products stands for 2^(-7 - e) of the score; of heads 2 quad and 2 quad + 1 (column c is held by lanes 4 c ..)
+    float back[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) back[e] = scale_log2 * 128.f * (1.f / __shfl_sync(0xffffffffu, down, 4 * (2 * quad + e)));
 
     float o[2 * NG][4];
 #pragma unroll
@@ -224,16 +244,16 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             const Words<kPairs> w0 = reinterpret_cast<const Words<kPairs>*>(words)[row], w1 = reinterpret_cast<const Words<kPairs>*>(words)[row + 8];
             {
                 const uint32_t a = words[row * kPairs + my_pair], c = words[(row + 8) * kPairs + my_pair];
-                const uint32_t za = mul_bf16x2(sub_bf16x2((a & 0x000f000fu) | 0x43004300u, 0x43004300u), a & 0xfff0fff0u);
-                const uint32_t zc = mul_bf16x2(sub_bf16x2((c & 0x000f000fu) | 0x43004300u, 0x43004300u), c & 0xfff0fff0u);
-                s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
-                mma16816(s[b], za, zc, za, zc, sums0, sums1);
+                const uint32_t za = mul_bf16x2(mul_bf16x2(a & 0x000f000fu, k2p127), a & 0xfff0fff0u);
+                const uint32_t zc = mul_bf16x2(mul_bf16x2(c & 0x000f000fu, k2p127), c & 0xfff0fff0u);
+                mma16816_0(s[b], za, zc, za, zc, sums0, sums1);
             }
 #pragma unroll
             for (int k = 0; k < NG; ++k) {
-                float acc[4] = {start[k][0], start[k][1], start[k][0], start[k][1]};
-                mma16816(acc, pair128(c0.w[k], 0), pair128(c1.w[k], 0), pair128(c0.w[k], 1), pair128(c1.w[k], 1), qf[k][0], qf[k][1]);
-                mma16816(acc, pair128(c0.w[k], 2), pair128(c1.w[k], 2), pair128(c0.w[k], 3), pair128(c1.w[k], 3), qf[k][2], qf[k][3]);
+                float acc[4];
+                const uint32_t x0 = c0.w[k], x1 = c1.w[k], y0 = x0 >> 8, y1 = x1 >> 8;
+                mma16816_0(acc, x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u, qf[k][0], qf[k][1]);
+                mma16816(acc, y0 & 0x000f000fu, y1 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x00f000f0u, qf[k][2], qf[k][3]);
                 const uint32_t a = w0.w[k >> 1], c = w1.w[k >> 1];
                 const float sa = __uint_as_float((k & 1 ? a : a << 16) & 0xfff00000u), sc = __uint_as_float((k & 1 ? c : c << 16) & 0xfff00000u);
                 s[b][0] = fmaf(sa, acc[0], s[b][0]);
@@ -241,6 +261,8 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
                 s[b][2] = fmaf(sc, acc[2], s[b][2]);
                 s[b][3] = fmaf(sc, acc[3], s[b][3]);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[b][e] *= back[e & 1];
         }
         bool seen[2][2] = {{true, true}, {true, true}};
         if (!whole) {
@@ -257,11 +279,11 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
         float top[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            float x = fmaxf(fmaxf(s[0][e], s[0][2 + e]), fmaxf(s[1][e], s[1][2 + e])) ;
+            float x = fmaxf(fmaxf(s[0][e], s[0][2 + e]), fmaxf(s[1][e], s[1][2 + e]));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-            top[e] = fmaxf(m[e], x * scale_log2);
+            top[e] = fmaxf(m[e], x);
         }
         if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
             float corr[2];
@@ -281,7 +303,7 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             float p[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                p[e] = ex2(fmaf(s[b][e], scale_log2, -base[e & 1]));
+                p[e] = ex2(s[b][e] - base[e & 1]);
                 l[e & 1] += p[e];
             }
             const unsigned char* block = stage + b * kBytes;
@@ -298,11 +320,14 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
                     sc = seen[b][1] ? sc : 0.f;
                 }
                 const uint32_t b0 = transpose8(pack_bf16(p[0] * sa, p[1] * sa)), b1 = transpose8(pack_bf16(p[2] * sc, p[3] * sc));
-                const uint32_t za = (z0.w[k] & 0x000f000fu) | 0x43004300u, zc = (z1.w[k] & 0x000f000fu) | 0x43004300u;
+                const uint32_t za = mul_bf16x2(z0.w[k] & 0x000f000fu, kMinus2p127), zc = mul_bf16x2(z1.w[k] & 0x000f000fu, kMinus2p127);
+                uint32_t x0 = v0.w[k], x1 = v1.w[k];
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-                    mma16816(o[2 * k + t], sub_bf16x2(pair128(v0.w[k], 2 * t), za), sub_bf16x2(pair128(v0.w[k], 2 * t + 1), za),
-                             sub_bf16x2(pair128(v1.w[k], 2 * t), zc), sub_bf16x2(pair128(v1.w[k], 2 * t + 1), zc), b0, b1);
+                for (int t = 0; t < 2; ++t) {
+                    mma16816(o[2 * k + t], fma_bf16x2(x0 & 0x000f000fu, k2p127, za), fma_bf16x2(x0 & 0x00f000f0u, k2p123, za),
+                             fma_bf16x2(x1 & 0x000f000fu, k2p127, zc), fma_bf16x2(x1 & 0x00f000f0u, k2p123, zc), b0, b1);
+                    x0 >>= 8, x1 >>= 8;
+                }
             }
         }
     }
@@ -335,6 +360,7 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             L += sm_l[w * kDecHeads + h] * f;
             O += sm_o[(size_t)(w * kDecHeads + h) * D + x] * f;
         }
+        O *= 64.f;                              // (the operands were (code - zero) 2^-6)
         if (alone) {
             out[(size_t)token * out_stride + (size_t)(head0 + h) * D + x] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L);
         } else {
