@@ -15,12 +15,18 @@
 // two a head, so that their largest lies in [2^126, 2^127), and by 1/16 against the codes of bits 4-7; the scores take it back.
 // The zero points of all groups are one more MMA with step * zero (four bits times four) against the sums of q, which are split into
 // bfloat16 parts.  All operands of the scores are exact.  For the values one fused multiply-add on the other pipe gives (code - zero) 2^-6,
-// also exact; only p * step is rounded, once.  The weights come out of the scores with keys as rows and go in with keys as the summed
-// index: one 8 x 8 transposition in registers (movmatrix) for 8 keys.
+// also exact; only p * step is rounded, once: p enters that product as two bfloat16 parts.  The weights come out of the scores with keys as rows
+// and go in with keys as the summed index: an 8 x 8 transposition in registers (movmatrix) for 8 keys and part.
 //
-// A running maximum and sum per head in base 2, in 32 bits; warps are merged in shared memory, CTAs by a second kernel from partial results in
-// scratch memory that the caller brings: [(request, head)][split][D] and [..][2] (nothing global is counted or kept, so any
-// number of launches may run at once).
+// A running maximum and sum per head in base 2, in 32 bits; the warps of a CTA are merged in shared memory.
+//
+// The work of a launch is one list: the blocks of request 0, head block 0, then head block 1, .. , request 1, .., in units of `unit`
+// blocks.  The launch has as many CTAs as the GPU holds at once and every CTA takes the same number of consecutive units, found from the
+// lengths on the device: requests of any lengths end together, and a recorded launch fits whatever lengths it is replayed with.
+// What a CTA has of a (request, head block) goes straight to the output if it is all of it; else it is a partial result: its first or its
+// last piece, so two places a CTA in scratch memory that the caller brings hold them all, and a second kernel joins them (nothing global is
+// counted or kept, so any number of launches may run at once).  64 requests of 1 024 to 8 192 tokens, 32 heads over 8: equal numbers of
+// splits for every request left the SMs idle a third of the time.
 #include "kv4.cuh"
 #include "mma_utils.cuh"
 #include "tcgen05_utils.cuh"
@@ -37,18 +43,57 @@ constexpr int stage_bytes() { return 2 * block_bytes(D); }
 template <int D>
 constexpr int ring_bytes() { return kDecWarps * kDecStages * stage_bytes<D>(); }
 
-// the blocks [first, first + count) of a request that its last token sees, and how many of them a CTA takes
+// The blocks [first, first + count) of a request that its last token sees.
 struct Span {
-    int first, count, chunk;
+    int first, count;
 };
-__device__ __forceinline__ Span span_of(int seq_len, int window, int splits) {
-    Span s;
+__device__ __forceinline__ Span span_of(int seq_len, int window) {
     const int lo = window > 0 ? max(0, seq_len - window) : 0;
-    s.first = lo / kBlock;
-    s.count = max(0, (seq_len + kBlock - 1) / kBlock - s.first);
-    constexpr int unit = 2 * kDecWarps;                          // two blocks for every warp
-    s.chunk = max(1, (s.count + splits * unit - 1) / (splits * unit)) * unit;
-    return s;
+    const int first = lo / kBlock;
+    return {first, max(0, (int)(((long long)seq_len + kBlock - 1) / kBlock) - first)};
+}
+// Units of a request for each head block; a single token without keys has one too (its row is zero), other requests none.
+__device__ __forceinline__ int units_of(int r, const int* query_start_loc, const int* seq_lens, int window, int unit) {
+    if (query_start_loc[r + 1] - query_start_loc[r] != 1) return 0;
+    return max(1, (span_of(seq_lens[r], window).count + unit - 1) / unit);
+}
+// Where the list of units stands: a warp sums up the requests' units and finds the request that unit `at` of head block 0.. lies in.
+struct Place {
+    long long total, before;         // all units; those of the requests in front of `request`
+    int request;
+};
+__device__ __forceinline__ Place warp_find(long long at_part, int parts, int num_requests, const int* query_start_loc, const int* seq_lens, int window,
+                                           int unit, int head_blocks) {
+    const int lane = threadIdx.x & 31;
+    Place p{0, 0, num_requests};
+    for (int r0 = 0; r0 < num_requests; r0 += 32) {
+        const int r = r0 + lane;
+        long long n = r < num_requests ? (long long)units_of(r, query_start_loc, seq_lens, window, unit) * head_blocks : 0;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
+        p.total += n;
+    }
+    const long long share = (p.total + parts - 1) / parts, at = at_part * share;
+    long long before = 0;
+    for (int r0 = 0; r0 < num_requests && at < p.total; r0 += 32) {
+        const int r = r0 + lane;
+        long long upto = r < num_requests ? (long long)units_of(r, query_start_loc, seq_lens, window, unit) * head_blocks : 0;
+        const long long own = upto;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long o = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += o;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, before + upto > at);
+        if (hit) {
+            const int first = __ffs(hit) - 1;
+            p.request = r0 + first;
+            p.before = before + __shfl_sync(0xffffffffu, upto - own, first);
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return p;
 }
 
 template <int N>
@@ -91,39 +136,60 @@ template <int D>
 __global__ void __launch_bounds__(kDecWarps * 32, D > 128 ? 2 : 4)
 attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* __restrict__ out, int out_stride,
                         const unsigned char* __restrict__ cache, int num_pages, int page_size, const int* __restrict__ block_table, int table_stride,
-                        const int* __restrict__ query_start_loc, const int* __restrict__ seq_lens, int nq, int nkv, float scale_log2, int window,
-                        int splits, float* __restrict__ part_o, float* __restrict__ part_ml, int* __restrict__ error_flag) {
+                        const int* __restrict__ query_start_loc, const int* __restrict__ seq_lens, int num_requests, int nq, int nkv, float scale_log2, int window,
+                        int unit, float* __restrict__ part_o, float* __restrict__ part_ml, int* __restrict__ error_flag) {
     constexpr int NG = D / kGroup;
     constexpr int kBytes = block_bytes(D);
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint64_t s_full[kDecWarps * kDecStages];
+    __shared__ Place s_place;
+    __shared__ int s_failed;         // a wait ran out: no further one is begun
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, row = lane >> 2;
-    const int split = blockIdx.x, r = blockIdx.z;
-    const int g = nq / nkv, head_blocks = (g + kDecHeads - 1) / kDecHeads;
-    const int kvh = blockIdx.y / head_blocks, hb = blockIdx.y - kvh * head_blocks;
-    const int head0 = kvh * g + hb * kDecHeads, nh = min(kDecHeads, g - hb * kDecHeads);
+    const int g = nq / nkv, blocks_per_kv = (g + kDecHeads - 1) / kDecHeads, head_blocks = nkv * blocks_per_kv;
 
     if (lane < kDecStages) mbar_init(&s_full[warp * kDecStages + lane], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    const int token = query_start_loc[r];
-    const bool mine = query_start_loc[r + 1] - token == 1;
-    const int seq_len = seq_lens[r];
+    if (warp == 0) {
+        const Place p = warp_find(blockIdx.x, gridDim.x, num_requests, query_start_loc, seq_lens, window, unit, head_blocks);
+        if (lane == 0) s_place = p, s_failed = 0;
+    }
+    __syncthreads();
     griddep_wait();          // queries and this step's keys and values come from the kernel before
     griddep_launch();
-    if (!mine) return;
-    const Span span = span_of(seq_len, window, splits);
-    if (split != 0 && split * span.chunk >= span.count) return;
-    const bool alone = span.chunk >= span.count;
-    const int begin = span.first + split * span.chunk, end = min(span.first + span.count, begin + span.chunk);
-    const int lo = window > 0 ? max(0, seq_len - window) : 0;
-    const int* table = block_table + (size_t)r * table_stride;
+    const Place place = s_place;
+    const long long share = (place.total + gridDim.x - 1) / gridDim.x;
+    const long long from = blockIdx.x * share, to = min(place.total, from + share);
     const int per_page = page_size / kBlock;
-
-    // this warp's pairs of blocks: begin + 2 (i * warps + warp), i = 0 .. mine_pairs - 1
-    const int pairs = (end - begin + 1) / 2;
-    const int count = pairs > warp ? (pairs - warp + kDecWarps - 1) / kDecWarps : 0;
     unsigned char* ring = smem + warp * kDecStages * stage_bytes<D>();
     uint64_t* full = s_full + warp * kDecStages;
+    int st = 0;                      // the ring stage that is read next, and the parity of its barrier
+    uint32_t parity = 0;
+    long long before = place.before, at = from;
+    int r = place.request;
+
+    while (at < to) {
+    int units = units_of(r, query_start_loc, seq_lens, window, unit);
+    while (at >= before + (long long)units * head_blocks) {
+        before += (long long)units * head_blocks;
+        units = units_of(++r, query_start_loc, seq_lens, window, unit);
+    }
+    const int local = (int)(at - before), hblock = local / units, u0 = local - hblock * units;
+    const int u1 = (int)min((long long)units, u0 + (to - at));
+    const bool first_piece = at == from;
+    at += u1 - u0;
+    const bool alone = u0 == 0 && u1 == units;
+    const int kvh = hblock / blocks_per_kv, hb = hblock - kvh * blocks_per_kv;
+    const int head0 = kvh * g + hb * kDecHeads, nh = min(kDecHeads, g - hb * kDecHeads);
+    const int token = query_start_loc[r];
+    const int seq_len = seq_lens[r];
+    const Span span = span_of(seq_len, window);
+    const int begin = span.first + u0 * unit, end = span.first + min(span.count, u1 * unit);
+    const int lo = window > 0 ? max(0, seq_len - window) : 0;
+    const int* table = block_table + (size_t)r * table_stride;
+
+    // this warp's pairs of blocks: begin + 2 (i * warps + warp), i = 0 .. count - 1
+    const int pairs = (end - begin + 1) / 2;
+    const int count = pairs > warp ? (pairs - warp + kDecWarps - 1) / kDecWarps : 0;
     // lanes 2 j and 2 j + 1 look up the blocks of pair 16 n + j, a batch of 16 pairs ahead of its use
     auto lookup = [&](int batch) {
         const int i = batch * 16 + (lane >> 1);
@@ -135,25 +201,28 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
         return page >= 0 && page < num_pages ? (page * nkv + kvh) * per_page + (b - index * per_page) : -1;
     };
     int ids = lookup(0), ids_next = lookup(1);
-    uint32_t present = 0;            // two bits a ring stage: which of its blocks the table names
-    auto request = [&](int i) {
+    uint32_t named = __ballot_sync(0xffffffffu, ids >= 0);       // two bits a pair of the batch: which of its blocks the table names
+    uint32_t present = 0;                                        // the same of the pairs on their way, the oldest in the lowest bits
+    int fill = st;
+    auto request = [&](int i, int in_flight) {
         if (i != 0 && (i & 15) == 0) {
             ids = ids_next;
             ids_next = lookup((i >> 4) + 1);
+            named = __ballot_sync(0xffffffffu, ids >= 0);
         }
-        const int s = i % kDecStages;
-        const uint32_t here = (__ballot_sync(0xffffffffu, ids >= 0) >> (2 * (i & 15))) & 3u;
-        present = (present & ~(3u << (2 * s))) | (here << (2 * s));
-        if (lane == 0) mbar_expect_tx(&full[s], __popc(here) * kBytes);
+        const uint32_t here = (named >> (2 * (i & 15))) & 3u;
+        present |= here << (2 * in_flight);
+        if (lane == 0) mbar_expect_tx(&full[fill], __popc(here) * kBytes);
         __syncwarp();
         if ((lane >> 1) == (i & 15) && ids >= 0)
-            bulk_load(ring + s * stage_bytes<D>() + (lane & 1) * kBytes, cache + (size_t)ids * kBytes, kBytes, &full[s]);
+            bulk_load(ring + fill * stage_bytes<D>() + (lane & 1) * kBytes, cache + (size_t)ids * kBytes, kBytes, &full[fill]);
+        fill = fill == kDecStages - 1 ? 0 : fill + 1;
     };
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < kDecStages - 1; ++i)
-        if (i < count) request(i);
+    for (int i = 0; i < kDecStages - 2; ++i)
+        if (i < count) request(i, i);
 
     // ---- queries: the B operand, head = column `row`; a lane has values 32 g + 8 quad .. + 7 of every group ----
     uint32_t qf[NG][4];
@@ -218,24 +287,19 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
     for (int i = 0; i < 2 * NG; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-    for (int i = 0; i < count; ++i) {
-        const int st = i % kDecStages;
-        const bool landed = __all_sync(0xffffffffu, mbar_wait(&full[st], (uint32_t)((i / kDecStages) & 1)));
-        if (!landed) {
-            if (lane == 0) atomicExch(error_flag, 41);
-            break;
-        }
-        // the stage that pair i - 1 was read from is refilled: every lane has finished reading it
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (i + kDecStages - 1 < count) request(i + kDecStages - 1);
-        const unsigned char* stage = ring + st * stage_bytes<D>();
-        const int block0 = begin + 2 * (i * kDecWarps + warp);
-        const uint32_t here = (present >> (2 * st)) & 3u;
+    // ---- scores of the 32 keys of a stage, scaled; keys that are not seen: -inf, and their values' words cleared (what lies where no token
+    // has been written may be anything) ----
+    auto scores = [&](unsigned char* stage, int block0, uint32_t here, float (&s)[2][4]) {
         const bool whole = here == 3u && block0 * kBlock >= lo && (block0 + 2) * kBlock <= seq_len;
-
-        // ---- scores of 32 keys ----
-        float s[2][4];
+        if (!whole) {
+            const int key = block0 * kBlock + lane;
+            if (!((here >> (lane >> 4)) & 1u) || key < lo || key >= seq_len) {
+                uint16_t* words = reinterpret_cast<uint16_t*>(stage + (lane >> 4) * kBytes + value_words_at(D)) + ((lane & 15) >> 1) * NG * 2 + (lane & 1);
+#pragma unroll
+                for (int k = 0; k < NG; ++k) words[2 * k] = 0;
+            }
+            __syncwarp();
+        }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const unsigned char* block = stage + b * kBytes;
@@ -264,18 +328,43 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[b][e] *= back[e & 1];
         }
-        bool seen[2][2] = {{true, true}, {true, true}};
         if (!whole) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int key = (block0 + b) * kBlock + row + 8 * h;
-                    seen[b][h] = ((here >> b) & 1u) && key >= lo && key < seq_len;
-                    if (!seen[b][h]) s[b][2 * h] = s[b][2 * h + 1] = -INFINITY;
+                    if (!((here >> b) & 1u) || key < lo || key >= seq_len) s[b][2 * h] = s[b][2 * h + 1] = -INFINITY;
                 }
         }
-        // ---- running maximum; heads 2 quad (e = 0) and 2 quad + 1 ----
+    };
+    // ---- O += (p step) (code - zero) of a stage.  p enters as two bfloat16 parts, so that only p * step is rounded (2^-9 of it; what the parts
+    // leave out is 2^-18) ----
+    auto values = [&](const unsigned char* stage, const uint32_t (&ph)[2][2], const uint32_t (&pl)[2][2]) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const unsigned char* block = stage + b * kBytes;
+            const Words<NG>* words = reinterpret_cast<const Words<NG>*>(block + value_words_at(D));
+            const Words<NG> z0 = words[quad], z1 = words[4 + quad];
+            const Words<NG>* codes = reinterpret_cast<const Words<NG>*>(block + value_codes_at(D));
+            const Words<NG> v0 = codes[lane], v1 = codes[32 + lane];
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+                const uint32_t sa = z0.w[k] & 0xfff0fff0u, sc = z1.w[k] & 0xfff0fff0u;
+                const uint32_t b0 = fma_bf16x2(ph[b][0], sa, mul_bf16x2(pl[b][0], sa)), b1 = fma_bf16x2(ph[b][1], sc, mul_bf16x2(pl[b][1], sc));
+                const uint32_t za = mul_bf16x2(z0.w[k] & 0x000f000fu, kMinus2p127), zc = mul_bf16x2(z1.w[k] & 0x000f000fu, kMinus2p127);
+                uint32_t x0 = v0.w[k], x1 = v1.w[k];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    mma16816(o[2 * k + t], fma_bf16x2(x0 & 0x000f000fu, k2p127, za), fma_bf16x2(x0 & 0x00f000f0u, k2p123, za),
+                             fma_bf16x2(x1 & 0x000f000fu, k2p127, zc), fma_bf16x2(x1 & 0x00f000f0u, k2p123, zc), b0, b1);
+                    x0 >>= 8, x1 >>= 8;
+                }
+            }
+        }
+    };
+    // weights of a stage's scores: running maximum (heads 2 quad, e = 0, and 2 quad + 1), sums, and the transposed parts of p
+    auto weigh = [&](const float (&s)[2][4], uint32_t (&ph)[2][2], uint32_t (&pl)[2][2]) {
         float top[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -297,39 +386,55 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             for (int t = 0; t < 2 * NG; ++t) o[t][0] *= corr[0], o[t][1] *= corr[1], o[t][2] *= corr[0], o[t][3] *= corr[1];
         }
         const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-        // ---- weights and values ----
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            float p[4];
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                p[e] = ex2(s[b][e] - base[e & 1]);
-                l[e & 1] += p[e];
+            for (int h = 0; h < 2; ++h) {
+                const float p0 = ex2(s[b][2 * h] - base[0]), p1 = ex2(s[b][2 * h + 1] - base[1]);
+                l[0] += p0, l[1] += p1;
+                const uint32_t hi = pack_bf16(p0, p1);
+                ph[b][h] = transpose8(hi);
+                pl[b][h] = transpose8(pack_bf16(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u)));
             }
-            const unsigned char* block = stage + b * kBytes;
-            const Words<NG>* words = reinterpret_cast<const Words<NG>*>(block + value_words_at(D));
-            const Words<NG> a0 = words[row >> 1], a1 = words[4 + (row >> 1)], z0 = words[quad], z1 = words[4 + quad];
-            const Words<NG>* codes = reinterpret_cast<const Words<NG>*>(block + value_codes_at(D));
-            const Words<NG> v0 = codes[lane], v1 = codes[32 + lane];
-            const int up = row & 1 ? 0 : 16;
-#pragma unroll
-            for (int k = 0; k < NG; ++k) {
-                float sa = __uint_as_float((a0.w[k] << up) & 0xfff00000u), sc = __uint_as_float((a1.w[k] << up) & 0xfff00000u);
-                if (!whole) {                                   // what lies where no token has been written may be anything
-                    sa = seen[b][0] ? sa : 0.f;
-                    sc = seen[b][1] ? sc : 0.f;
-                }
-                const uint32_t b0 = transpose8(pack_bf16(p[0] * sa, p[1] * sa)), b1 = transpose8(pack_bf16(p[2] * sc, p[3] * sc));
-                const uint32_t za = mul_bf16x2(z0.w[k] & 0x000f000fu, kMinus2p127), zc = mul_bf16x2(z1.w[k] & 0x000f000fu, kMinus2p127);
-                uint32_t x0 = v0.w[k], x1 = v1.w[k];
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    mma16816(o[2 * k + t], fma_bf16x2(x0 & 0x000f000fu, k2p127, za), fma_bf16x2(x0 & 0x00f000f0u, k2p123, za),
-                             fma_bf16x2(x1 & 0x000f000fu, k2p127, zc), fma_bf16x2(x1 & 0x00f000f0u, k2p123, zc), b0, b1);
-                    x0 >>= 8, x1 >>= 8;
-                }
-            }
+    };
+    // stage i has landed (false: the wait ran out); the stage that pair i - 2 was read from is refilled
+    auto arrive = [&](int i) {
+        bool landed = mbar_try_wait(&full[st], parity);
+        if (!landed) landed = *(volatile int*)&s_failed == 0 && mbar_wait(&full[st], parity);
+        if (!__all_sync(0xffffffffu, landed)) {
+            if (lane == 0) atomicExch(error_flag, 41), *(volatile int*)&s_failed = 1;
+            return false;
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // (every lane has finished reading that stage)
+        __syncwarp();
+        if (i + kDecStages - 2 < count) request(i + kDecStages - 2, kDecStages - 2);
+        return true;
+    };
+    // The scores of pair i + 1 are computed beside the weighted sum of pair i: one is integer work and short of independent products,
+    // the other fused multiply-adds.
+    uint32_t ph[2][2], pl[2][2];
+    unsigned char* stage = ring + st * stage_bytes<D>();
+    if (count > 0) {
+        float s[2][4];
+        bool ok = arrive(0);
+        if (ok) {
+            scores(stage, begin + 2 * warp, present & 3u, s);
+            present >>= 2;
+            weigh(s, ph, pl);
+        }
+        for (int i = 1; i < count && ok; ++i) {
+            const unsigned char* last = stage;
+            if (++st == kDecStages) st = 0, parity ^= 1u;
+            stage = ring + st * stage_bytes<D>();
+            ok = arrive(i);
+            if (!ok) break;
+            scores(stage, begin + 2 * (i * kDecWarps + warp), present & 3u, s);
+            present >>= 2;
+            values(last, ph, pl);
+            weigh(s, ph, pl);
+        }
+        if (ok) values(stage, ph, pl);
+        if (++st == kDecStages) st = 0, parity ^= 1u;
     }
     __syncthreads();     // all rings have been read
     // ---- merge the warps: [warp][head][D] values, [warp][head] maxima and sums ----
@@ -364,36 +469,60 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
         if (alone) {
             out[(size_t)token * out_stride + (size_t)(head0 + h) * D + x] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L);
         } else {
-            const size_t at = ((size_t)r * nq + head0 + h) * splits + split;
-            part_o[at * D + x] = O;
-            if (x == 0) part_ml[at * 2] = M, part_ml[at * 2 + 1] = L;
+            const size_t place = ((size_t)blockIdx.x * 2 + (first_piece ? 0 : 1)) * kDecHeads + h;
+            part_o[place * D + x] = O;
+            if (x == 0) part_ml[place * 2] = M, part_ml[place * 2 + 1] = L;
         }
+    }
+    __syncthreads();     // (the rings are filled again)
     }
 }
 
-// A CTA per (request, query head), a thread per value.
+// A CTA per (head, request), a thread per value: joins what several CTAs have of it.
 template <int D>
 __global__ void __launch_bounds__(D)
 attention_decode_merge_kernel(__nv_bfloat16* __restrict__ out, int out_stride, const int* __restrict__ query_start_loc, const int* __restrict__ seq_lens,
-                              int nq, int window, int splits, const float* __restrict__ part_o, const float* __restrict__ part_ml) {
+                              int num_requests, int nq, int nkv, int window, int unit, int parts, const float* __restrict__ part_o,
+                              const float* __restrict__ part_ml) {
+    __shared__ long long s_total[2];
     const int head = blockIdx.x, r = blockIdx.y, x = threadIdx.x;
-    const int token = query_start_loc[r];
-    const bool mine = query_start_loc[r + 1] - token == 1;
-    const Span span = span_of(seq_lens[r], window, splits);
+    const int g = nq / nkv, blocks_per_kv = (g + kDecHeads - 1) / kDecHeads, head_blocks = nkv * blocks_per_kv;
+    if (threadIdx.x < 32) {
+        long long total = 0, before = 0;
+        for (int i = threadIdx.x; i < num_requests; i += 32) {
+            const long long n = (long long)units_of(i, query_start_loc, seq_lens, window, unit) * head_blocks;
+            total += n;
+            before += i < r ? n : 0;
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+            total += __shfl_xor_sync(0xffffffffu, total, d);
+            before += __shfl_xor_sync(0xffffffffu, before, d);
+        }
+        if (threadIdx.x == 0) s_total[0] = total, s_total[1] = before;
+    }
+    __syncthreads();
     griddep_wait();
     griddep_launch();
-    if (!mine || span.chunk >= span.count) return;
-    const int active = (span.count + span.chunk - 1) / span.chunk;
-    const size_t at = ((size_t)r * nq + head) * splits;
+    const int units = units_of(r, query_start_loc, seq_lens, window, unit);
+    if (units == 0) return;
+    const int kvh = head / g, in_kv = head - kvh * g, hblock = kvh * blocks_per_kv + in_kv / kDecHeads, h = in_kv % kDecHeads;
+    const long long share = (s_total[0] + parts - 1) / parts, from = s_total[1] + (long long)hblock * units, to = from + units;
+    const int c0 = (int)(from / share), c1 = (int)((to - 1) / share);
+    if (c0 == c1) return;
+    // the first CTA has it as its last piece, unless it is also its first; all others as their first
+    auto place_of = [&](int c) { return ((size_t)c * 2 + (c == c0 && from != c0 * share ? 1 : 0)) * kDecHeads + h; };
     float M = -INFINITY, L = 0.f, O = 0.f;
-    for (int s = 0; s < active; ++s) M = fmaxf(M, part_ml[(at + s) * 2]);
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) M = fmaxf(M, part_ml[place_of(c) * 2]);
 #pragma unroll 8
-    for (int s = 0; s < active; ++s) {
-        const float m = part_ml[(at + s) * 2], f = m == -INFINITY ? 0.f : ex2(m - M);
-        L += part_ml[(at + s) * 2 + 1] * f;
-        O += part_o[(at + s) * D + x] * f;
+    for (int c = c0; c <= c1; ++c) {
+        const size_t place = place_of(c);
+        const float m = part_ml[place * 2], f = m == -INFINITY ? 0.f : ex2(m - M);
+        L += part_ml[place * 2 + 1] * f;
+        O += part_o[place * D + x] * f;
     }
-    out[(size_t)token * out_stride + (size_t)head * D + x] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L);
+    out[(size_t)query_start_loc[r] * out_stride + (size_t)head * D + x] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L);
 }
 
 }  // namespace kv4
@@ -405,35 +534,39 @@ extern "C" int cib_attention_kv4_decode_supports(int d, int page_size) {
     return kv4::sizes_ok(d, page_size) && (d == 64 || d == 128 || d == 256);
 }
 
-// Computes the rows of the requests that bring one token; the others' are left as they are.  scratch: splits * requests * nq * (d + 2)
-// floats where splits > 1.
+// As many CTAs as an SM holds: shared memory for 4 at head size 128, registers below.
+extern "C" int cib_attention_kv4_decode_ctas(int d) { return 148 * (d > 128 ? 2 : 4); }
+extern "C" long long cib_attention_kv4_decode_scratch_floats(int d, int ctas) { return (long long)ctas * 2 * kv4::kDecHeads * (d + 2); }
+
+// Computes the rows of the requests that bring one token; the others' are left as they are.  ctas: how many CTAs share the work; unit: blocks
+// of 16 keys that a CTA has at least.  scratch: cib_attention_kv4_decode_scratch_floats, or none where no request has more than `unit`
+// blocks (no request is split then, whatever its length).
 extern "C" int cib_attention_kv4_decode(const void* q, int q_stride, void* out, int out_stride, const void* cache, int num_pages, int page_size,
                                         const int* block_table, int table_stride, const int* query_start_loc, const int* seq_lens, int num_requests, int nq,
-                                        int nkv, int d, float scale, int window, int splits, float* scratch, int* error_flag, int use_pdl, cudaStream_t stream) {
+                                        int nkv, int d, float scale, int window, int ctas, int unit, float* scratch, int* error_flag, int use_pdl,
+                                        cudaStream_t stream) {
     CIB_REQUIRE(cib_attention_kv4_decode_supports(d, page_size), "attention_kv4_decode: head size %d (64, 128 or 256), page size %d (a multiple of 16) are not taken", d, page_size);
     CIB_REQUIRE(num_requests >= 0 && num_requests <= 65535 && nq > 0 && nkv > 0 && nq % nkv == 0, "attention_kv4_decode: bad sizes R=%d nq=%d nkv=%d", num_requests, nq, nkv);
-    CIB_REQUIRE(splits >= 1 && (splits == 1 || scratch != nullptr), "attention_kv4_decode: scratch missing");
+    CIB_REQUIRE(ctas >= 1 && unit >= 1 && unit <= 1 << 20, "attention_kv4_decode: bad launch shape %d, %d", ctas, unit);
     CIB_REQUIRE(num_pages > 0 && table_stride > 0 && cache != nullptr && ((uintptr_t)cache % 16) == 0, "attention_kv4_decode: bad cache geometry");
     CIB_REQUIRE((long long)num_pages * nkv * (page_size / kv4::kBlock) < (1ll << 31), "attention_kv4_decode: more than 2^31 blocks");
     CIB_REQUIRE(q_stride % 8 == 0 && ((uintptr_t)q % 16) == 0, "attention_kv4_decode: query rows must be 16-byte aligned");
     CIB_REQUIRE(window >= 0 && error_flag != nullptr, "attention_kv4_decode: window must be >= 0, error flag given");
-    const int g = nq / nkv, head_blocks = (g + kv4::kDecHeads - 1) / kv4::kDecHeads;
-    CIB_REQUIRE((long long)nkv * head_blocks <= 65535, "attention_kv4_decode: too many heads");
     if (num_requests == 0) return 0;
     const float scale_log2 = scale * 1.4426950408889634f;
-    float* part_ml = scratch == nullptr ? nullptr : scratch + (size_t)num_requests * nq * splits * d;
-    const dim3 grid(splits, nkv * head_blocks, num_requests);
+    if (scratch == nullptr) unit = 1 << 27;          // a request is one unit, so no CTA has a part of it
+    float* part_ml = scratch == nullptr ? nullptr : scratch + (size_t)ctas * 2 * kv4::kDecHeads * d;
 #define CIB_KV4_DECODE(DV)                                                                                                                           \
     if (d == DV) {                                                                                                                                   \
         static SmemLimit limit;                                                                                                                      \
         if (int rc = raise_smem_limit(limit, kv4::attention_decode_kernel<DV>, kv4::ring_bytes<DV>(), "attention_kv4_decode")) return rc;            \
-        cudaError_t e = launch_pdl(kv4::attention_decode_kernel<DV>, grid, dim3(kv4::kDecWarps * 32), (size_t)kv4::ring_bytes<DV>(), stream,         \
+        cudaError_t e = launch_pdl(kv4::attention_decode_kernel<DV>, dim3(ctas), dim3(kv4::kDecWarps * 32), (size_t)kv4::ring_bytes<DV>(), stream,   \
                                    use_pdl != 0, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, (const unsigned char*)cache,     \
-                                   num_pages, page_size, block_table, table_stride, query_start_loc, seq_lens, nq, nkv, scale_log2, window, splits,   \
-                                   scratch, part_ml, error_flag);                                                                                    \
-        if (e == cudaSuccess && splits > 1)                                                                                                          \
+                                   num_pages, page_size, block_table, table_stride, query_start_loc, seq_lens, num_requests, nq, nkv, scale_log2,    \
+                                   window, unit, scratch, part_ml, error_flag);                                                                      \
+        if (e == cudaSuccess && scratch != nullptr)                                                                                                  \
             e = launch_pdl(kv4::attention_decode_merge_kernel<DV>, dim3(nq, num_requests), dim3(DV), 0, stream, use_pdl != 0, (__nv_bfloat16*)out,   \
-                           out_stride, query_start_loc, seq_lens, nq, window, splits, scratch, part_ml);                                             \
+                           out_stride, query_start_loc, seq_lens, num_requests, nq, nkv, window, unit, ctas, scratch, part_ml);                      \
         CIB_REQUIRE(e == cudaSuccess, "attention_kv4_decode: launch failed: %s", cudaGetErrorString(e));                                             \
         return 0;                                                                                                                                    \
     }

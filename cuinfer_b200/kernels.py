@@ -122,7 +122,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "cib_qk_norm_rope_kv4_write": [_P, _I, _I, _P, _I, _P, _P, _P, _P, _I, _I, _F, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P],
         "cib_kv4_read": [_P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
         "cib_attention_kv4_generic": [_P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
-        "cib_attention_kv4_decode": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _F, _I, _I, _P, _P, _I, _P],
+        "cib_attention_kv4_decode": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _P, _P, _I, _P],
         "cib_gemm_skinny": [_P, _I, _I, _I, _P, _I, _P, _P, _I, _P, _I, _F, _P, _P, _I, _I, _I, _I, _I, _P, ctypes.c_longlong, _P, _I, _P, _P, _P],
         "cib_gemm_tcgen05": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P, _I, _F, _P, _P, _I, _P, _P, _P],
         "cib_gemm_wstream": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _P, _I, _F, _P, _P, _I, _P, _P, _I, _P, ctypes.c_longlong, _I, _P, _P],
@@ -155,6 +155,10 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.cib_paged_attention_decode_supports.restype = _I
     lib.cib_attention_kv4_decode_supports.argtypes = [_I, _I]
     lib.cib_attention_kv4_decode_supports.restype = _I
+    lib.cib_attention_kv4_decode_ctas.argtypes = [_I]
+    lib.cib_attention_kv4_decode_ctas.restype = _I
+    lib.cib_attention_kv4_decode_scratch_floats.argtypes = [_I, _I]
+    lib.cib_attention_kv4_decode_scratch_floats.restype = ctypes.c_longlong
     lib.cib_gemm_tcgen05_supports.argtypes = [_I, _I, _I]
     lib.cib_gemm_tcgen05_supports.restype = _I
     lib.cib_gemm_tcgen05_stream_cols.argtypes = [_I, _I, _I]
@@ -895,10 +899,14 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
     # request may then bring a single token.
     if (dtype == BF16 and library().cib_attention_kv4_decode_supports(head_dim, page_size) and q_args[1] % 8 == 0 and q_args[0] % 16 == 0
             and (1 in query_lens_host or sum(query_lens_host) > T)):
-        splits = kv4_decode_splits(R * num_kv_heads * -(-(num_q_heads // num_kv_heads) // 8), min(max_seq_len, window or max_seq_len), head_dim)
-        scratch = torch.empty(splits * R * num_q_heads * (head_dim + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
-        rc = library().cib_attention_kv4_decode(*q_args, *out_args, *cache_args, R, num_q_heads, num_kv_heads, head_dim, float(scale), int(window), splits,
-                                                scratch.data_ptr() if scratch is not None else None, _error_flag(q.device).data_ptr(), pdl, _stream())
+        lib = library()
+        ctas, unit = kv4_decode_shape(R * num_kv_heads * -(-(num_q_heads // num_kv_heads) // 8), min(max_seq_len, window + 16 if window else max_seq_len),
+                                      lib.cib_attention_kv4_decode_ctas(head_dim))
+        scratch = None
+        if min(max_seq_len, window + 16 if window else max_seq_len) > unit * KV4_BLOCK:
+            scratch = torch.empty(lib.cib_attention_kv4_decode_scratch_floats(head_dim, ctas), dtype=torch.float32, device=q.device)
+        rc = lib.cib_attention_kv4_decode(*q_args, *out_args, *cache_args, R, num_q_heads, num_kv_heads, head_dim, float(scale), int(window), ctas, unit,
+                                          scratch.data_ptr() if scratch is not None else None, _error_flag(q.device).data_ptr(), pdl, _stream())
         _check(rc, who)
         note_flagged_launch()
         _count()
@@ -911,10 +919,11 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
     _count()
 
 
-def kv4_decode_splits(pairs: int, keys: int, head_dim: int) -> int:
-    """How many CTAs share the keys of a (request, kv head)."""
-    slots = 148 * (2 if head_dim > 128 else 4)
-    return max(1, min(64, -(-keys // 128), slots // pairs))
+def kv4_decode_shape(pairs: int, keys: int, slots: int) -> tuple:
+    """(CTAs, blocks of 16 keys that a CTA takes at least) of the 4-bit decode attention, for ``pairs`` (request, head block) of at most
+    ``keys`` keys on a GPU that holds ``slots`` of its CTAs: contexts of up to 512 keys are not split."""
+    unit = 32 if keys <= 512 else 8
+    return max(1, min(slots, pairs * -(-keys // (unit * KV4_BLOCK)))), unit
 
 
 # ---- matrix product ----------------------------------------------------------------------------------
