@@ -122,6 +122,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "cib_qk_norm_rope_kv4_write": [_P, _I, _I, _P, _I, _P, _P, _P, _P, _I, _I, _F, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P],
         "cib_kv4_read": [_P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
         "cib_attention_kv4_generic": [_P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
+        "cib_attention_kv4_prompt": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P],
         "cib_attention_kv4_decode": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _P, _P, _I, _P],
         "cib_gemm_skinny": [_P, _I, _I, _I, _P, _I, _P, _P, _I, _P, _I, _F, _P, _P, _I, _I, _I, _I, _I, _P, ctypes.c_longlong, _P, _I, _P, _P, _P],
         "cib_gemm_tcgen05": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P, _I, _F, _P, _P, _I, _P, _P, _P],
@@ -153,6 +154,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.cib_latent_attention_mma_tiles.restype = _I
     lib.cib_paged_attention_decode_supports.argtypes = [_I, _I, _I]
     lib.cib_paged_attention_decode_supports.restype = _I
+    lib.cib_attention_kv4_prompt_supports.argtypes = [_I, _I]
+    lib.cib_attention_kv4_prompt_supports.restype = _I
     lib.cib_attention_kv4_decode_supports.argtypes = [_I, _I]
     lib.cib_attention_kv4_decode_supports.restype = _I
     lib.cib_attention_kv4_decode_ctas.argtypes = [_I]
@@ -913,6 +916,20 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
         if T <= R and max(query_lens_host) <= 1:
             return
         least_query = 2
+    if (dtype == BF16 and library().cib_attention_kv4_prompt_supports(head_dim, page_size) and scale > 0
+            and q_args[1] % 8 == 0 and q_args[0] % 16 == 0 and out_args[1] % 8 == 0 and out_args[0] % 16 == 0):
+        g = num_q_heads // num_kv_heads
+        if sum(query_lens_host) > T:
+            pairs = T * g // 256 + R
+        else:
+            pairs = sum(-(-n * g // 256) for n in query_lens_host if n >= least_query)
+        folded = window <= 0 and pairs * num_kv_heads <= 148
+        rc = library().cib_attention_kv4_prompt(*q_args, *out_args, *cache_args, R, pairs, 1 if folded else 0, least_query, num_q_heads, num_kv_heads,
+                                                head_dim, float(scale), int(window), _error_flag(q.device).data_ptr(), _stream())
+        _check(rc, who)
+        note_flagged_launch()
+        _count()
+        return
     rc = library().cib_attention_kv4_generic(q_args[0], dtype, q_args[1], *out_args, *cache_args, T, R, max_seq_len, least_query, num_q_heads, num_kv_heads,
                                              head_dim, float(scale), int(window), pdl, _stream())
     _check(rc, who)

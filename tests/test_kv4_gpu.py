@@ -507,3 +507,60 @@ def test_generate_and_options(model_folders):
     assert llm.engine.runner.page_bytes() * 32 == plain.engine.runner.page_bytes() * 9
     with pytest.raises(ConfigError, match="does not take a cache in 4 bits"):
         LLM(model_folders["A"][0]["bfloat16"], block_size=16, num_blocks=64, kv_cache_dtype="int4")       # head size 16
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [64, 128, 96])
+@pytest.mark.parametrize("window", [0, 24])
+def test_a_later_value_that_is_no_number_does_not_reach_earlier_rows(dtype, d, window):
+    """A key that a row does not see may hold a value or a key that is not a number: its weight is zero, and zero times that is not."""
+    nq, nkv, lengths, new = 4, 2, [150, 90], [150, 70]
+    c = case(lengths, new, nq, nkv, d, 16, dtype, window=window, seed=12)
+    clean = attend(c).clone().reshape(-1, nkv, nq // nkv, d)
+    raw = c["cache"].cpu().numpy()
+    places = np.array(P4._places(d))
+    spots = [(0, 70, 0, 1, 33), (0, 71, 1, 1, 3), (0, 140, 0, 1, 40), (1, 50, 0, 0, 5), (1, 88, 1, 1, 34)]         # request, token, kv head, plane, value
+    for r, j, h, plane, i in spots:
+        at = places[j % 16, i, plane, 2]
+        block = raw[c["table"][r][j // 16], h, 0]
+        block[at], block[at + 1] = 0xF0, 0x7F
+    c["cache"] = torch.from_numpy(raw).to(DEV)
+    got = attend(c, torch.full((sum(new), nq * d), 5.0, dtype=dtype, device=DEV)).reshape(-1, nkv, nq // nkv, d)
+    for r, (n, fresh) in enumerate(zip(lengths, new)):
+        for i in range(fresh):
+            pos, row = n - fresh + i, c["starts"][r] + i
+            for h in range(nkv):
+                hit = torch.zeros(d, dtype=torch.bool)
+                for rr, j, hh, plane, value in spots:
+                    if rr == r and hh == h and j <= pos and (not window or j > pos - window):
+                        if plane == 0:
+                            hit[:] = True
+                        else:
+                            hit[value // 32 * 32:value // 32 * 32 + 32] = True
+                bad = torch.isnan(got[row, h]).cpu()
+                assert (bad == hit).all(), (r, i, h)
+                assert torch.equal(got[row, h].cpu()[~bad], clean[row, h].cpu()[~bad]), (r, i, h)
+
+
+@pytest.mark.parametrize("heads", [(2, 1, 128), (12, 4, 64), (5, 1, 128), (80, 2, 64), (8, 8, 128)])
+@pytest.mark.parametrize("shape", ["one long", "many", "portions", "bounds"])
+def test_prompts_of_many_row_tiles(heads, shape):
+    nq, nkv, d = heads
+    lengths, new = {"one long": ([700], [700]), "many": ([300, 270, 130, 257, 64, 65, 128, 129, 1, 2] * 2, [300, 270, 130, 257, 64, 65, 128, 129, 1, 2] * 2),
+                    "portions": ([900, 64, 700, 300], [300, 64, 1, 129]), "bounds": ([257, 257, 257, 1, 30], [257, 257, 257, 1, 2])}[shape]
+    if nq * sum(new) * max(lengths) > 12e6:
+        lengths, new = [min(n, 130) for n in lengths], [min(n, 130) for n in new]
+    c = case(lengths, new, nq, nkv, d, 16, BF16, seed=nq, spare_rows=3)
+    if shape == "bounds":
+        out = attend(c, lens=[sum(new) + 128] + [1] * (len(new) - 1), longest=5000)
+        check(c, out)
+    else:
+        check(c)
+
+
+def test_a_scale_that_is_not_positive():
+    for scale in (0.0, -0.1):
+        for new in (1, 40):
+            c = case([90, 70], [new, new], 4, 2, 128, 16, BF16, seed=3)
+            c["scale"] = scale
+            check(c)
