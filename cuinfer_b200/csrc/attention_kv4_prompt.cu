@@ -2,17 +2,18 @@
 //
 //   * A CTA has an SM alone and owns two tiles of 128 rows (query token x query head of one kv head) that walk the same 64-key tiles:
 //     what taking a key tile apart costs is shared by 256 rows.
-//   * Four warps take the codes apart: a warp's lanes read 16 bytes of codes each straight from global memory, a tile ahead, and write
-//     bfloat16 numbers into the tiles that the tensor cores read (128-byte swizzle).  step * (code - zero) is exact in bfloat16, so
-//     these are the cache's numbers.  Keys are a K-major operand, [key][value column]; values too, but transposed, [value column][key]: a
-//     word of value codes holds two neighbouring keys of a column, which is the order that operand has.
+//   * Eight warps take the codes apart, four the keys and four the values (four for both were the bottleneck: 2 450 cycles a key tile). Blocks
+//     come by bulk copies (`cp.async.bulk`, three key tiles ahead); a warp's lanes read 16 bytes of codes each and write bfloat16 numbers into
+//     the tiles that the tensor cores read (128-byte swizzle).  step * (code - zero) is exact in bfloat16, so these are the cache's
+//     numbers.  Keys are a K-major operand, [key][value column]; values too, but transposed, [value column][key]: a word of value codes
+//     holds two neighbouring keys of a column, which is the order that operand has.
 //   * S = Q K^T and O += P V are `tcgen05.mma.cta_group::1.kind::f16`, S, P and O in tensor memory (2 x (64 + 64 + 128) columns), issued by one
 //     thread; S of key tile j + 1 is computed while the softmax warps take the exponentials of tile j.
 //   * Eight softmax warps, a thread per row: running maximum in base 2 that is raised when it grows by more than 8 (or at all over the
 //     first 256 keys), the sum is of the rounded weights; P goes back over its scores in bfloat16.
 //   * Rows see the keys up to their position, the last `window` of them, and none of a page that the block table does not name.  A value that is not
-//     a number must not reach rows that do not see its key (0 x NaN is NaN): it is written as zero and noted, and the rows that see it
-//     get their NaN at the end.
+//     a number must not reach rows that do not see its key (0 x NaN is NaN): it is written as zero, and where a CTA has met one, its rows look
+//     through the words of the values that they see at the end.
 //
 // Which two tiles: neighbours where there are more CTAs than SMs (they see almost the same keys); else tile i and the last but i of a
 // request (`folded`), so that all CTAs of a launch that fits the GPU at once have the same work.
@@ -31,8 +32,9 @@ constexpr int kM = 128;               // rows of a tile
 constexpr int kN = 64;                // keys of a tile
 constexpr int kSoftWarps = 8;         // four to a row tile
 constexpr int kMmaWarp = kSoftWarps;
-constexpr int kTakeWarps = 4;         // take the codes apart
-constexpr int kThreads = (kSoftWarps + 1 + kTakeWarps) * 32;
+constexpr int kTakeWarps = 4;         // take the keys apart, and as many the values
+constexpr int kThreads = (kSoftWarps + 1 + 2 * kTakeWarps) * 32;
+constexpr int kRawStages = 4;         // key tiles as bytes: three on their way, one being read
 constexpr int kTmemCols = 512;        // per row tile: S of even key tiles | S of odd ones | O
 
 constexpr uint32_t kMinus2p127 = 0xff00ff00u, k2p127 = 0x7f007f00u, k2p123 = 0x7d007d00u, k64 = 0x42804280u;
@@ -48,6 +50,15 @@ struct alignas(N * 4) Words {
     uint32_t w[N];
 };
 
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// umma_desc_k_major_sw128 of an address in shared memory
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
+    return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
 // D = F32, A = B = BF16, both K-major, M = 128
 __host__ __device__ constexpr uint32_t idesc(int n) { return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t id, uint32_t acc) {
@@ -65,13 +76,19 @@ __device__ __forceinline__ void tst32(uint32_t taddr, const uint32_t (&r)[32]) {
           "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(tc_smem_u32(dst)), "l"(src), "r"(bytes), "r"(tc_smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ void tst_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <int D>
 struct Smem {
     static constexpr int kPanels = D / 64;                         // 64-column panels of a query or key row
     static constexpr int kQ = kPanels * kM * 128, kK = kPanels * kN * 128, kV = D * 128;
-    static constexpr int kBars = 2 * kQ + 2 * kK + 2 * kV;
+    static constexpr int kRawBlock = block_bytes(D) + 32;          // (padded: the four blocks of a tile start in different banks)
+    static constexpr int kRaw = 2 * kQ + 2 * kK + 2 * kV;
+    static constexpr int kBars = kRaw + kRawStages * (kN / kBlock) * kRawBlock;
     static constexpr int kTotal = kBars + 256 + 1024;
 };
 
@@ -95,13 +112,14 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
     uint64_t* s_full = bars + 4;        // [row tile][2] S of a key tile is in tensor memory: its keys' buffer is free
     uint64_t* p_ready = bars + 8;       // [row tile][2] P is (the softmax warps arrive)
     uint64_t* pv_done = bars + 12;      // [row tile][2] O includes a key tile: its values' buffer is free
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+    uint64_t* raw_full = bars + 16;     // [stages] a key tile's blocks have landed
+    uint64_t* raw_free = raw_full + kRawStages;     // [stages] the taking warps have read them
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_free + kRawStages);
     __shared__ int s_req, s_pair, s_abort, s_q0, s_n, s_seq;
-    // Which of a key tile's blocks the table does not name, tile j at j % 4: written once S of tile j - 2 is there, read up to P V of tile j.
-    __shared__ int s_missing[4];
-    // Values that are not numbers, per value buffer: the last tile that has any, plus one, and key by key that tile's number with its groups (8 bits)
-    // (a note is good for the tile that it names, so nothing is ever cleared).
-    __shared__ unsigned s_any[2], s_bad[2][kN];
+    // Which of a key tile's blocks the table does not name, tile j at j % 8: written three tiles ahead, when P V of tile j - 5 at least is done, and
+    // read up to P V of tile j.
+    __shared__ int s_missing[8];
+    __shared__ int s_odd;               // a value that is not a number has been met
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int kvh = blockIdx.x;         // heads vary fastest: every head's longest tiles start before any shorter ones
@@ -135,20 +153,19 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
         }
         if (lane == 0) {
             s_req = req, s_pair = pair, s_abort = 0;
-            s_any[0] = s_any[1] = 0;
+            s_odd = 0;
             if (req < num_requests) {
                 s_q0 = query_start_loc[req];
                 s_n = query_start_loc[req + 1] - query_start_loc[req];
                 s_seq = seq_lens[req];
             }
         }
-    } else if (warp == 1 && lane < 16) {
-        mbar_init(&bars[lane], lane < 4 ? kTakeWarps : lane >= 8 && lane < 12 ? 4 : 1);
+    } else if (warp == 1 && lane < 16 + 2 * kRawStages) {
+        mbar_init(&bars[lane], lane >= 16 + kRawStages ? 2 * kTakeWarps : lane < 4 || lane >= 16 ? kTakeWarps : lane >= 8 && lane < 12 ? 4 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (tid < 2 * kN) s_bad[tid / kN][tid % kN] = 0;
-    if (tid < 4) s_missing[tid] = 0;
+    if (tid < 8) s_missing[tid] = 0;
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem_u32(tmem_slot)), "r"((uint32_t)kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -206,23 +223,29 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
     if (warp <= kMmaWarp) asm volatile("bar.sync 10, %0;" ::"r"((kMmaWarp + 1) * 32) : "memory");
 
     auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
-        bool ok = *(volatile int*)&s_abort == 0 && mbar_wait(bar, parity);
+        bool ok = mbar_try_wait(bar, parity) || (*(volatile int*)&s_abort == 0 && mbar_wait(bar, parity));
         if (!ok && lane == 0) { atomicExch(error_flag, code); *(volatile int*)&s_abort = 1; }
         return __all_sync(0xffffffffu, ok) != 0;
     };
 
     if (active && warp == kMmaWarp) {
-        // ---- the MMAs: the whole warp walks the loop, lane 0 issues ----
+        // ---- the MMAs: the whole warp walks the loop, one lane issues.  Addresses are broadcast, so that the compiler knows them to be the
+        // warp's and keeps them in uniform registers (out of per-thread ones an MMA took 72 cycles to issue) ----
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint32_t aq = __shfl_sync(0xffffffffu, tc_smem_u32(sQ), 0), ak = __shfl_sync(0xffffffffu, tc_smem_u32(sK), 0), av = __shfl_sync(0xffffffffu, tc_smem_u32(sV), 0);
+        const bool elected = elect_one();
         auto issue_s = [&](int t, int j) {
-            if (lane != 0) return;
             const int b = j & 1;
-            const uint64_t qd = umma_desc_k_major_sw128(sQ + t * S::kQ), kd = umma_desc_k_major_sw128(sK + b * S::kK);
+            if (elected) {
+                const uint64_t qd = desc_k_major(aq + t * S::kQ), kd = desc_k_major(ak + b * S::kK);
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-                const uint64_t q_off = (uint64_t)(((k >> 2) * (kM * 128) + (k & 3) * 32) >> 4), k_off = (uint64_t)(((k >> 2) * (kN * 128) + (k & 3) * 32) >> 4);
-                umma_bf16(tmem + (uint32_t)(t * 256 + b * kN), qd + q_off, kd + k_off, idesc(kN), k != 0);
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint64_t q_off = (uint64_t)(((k >> 2) * (kM * 128) + (k & 3) * 32) >> 4), k_off = (uint64_t)(((k >> 2) * (kN * 128) + (k & 3) * 32) >> 4);
+                    umma_bf16(tm + (uint32_t)(t * 256 + b * kN), qd + q_off, kd + k_off, idesc(kN), k != 0);
+                }
+                umma_commit(&s_full[t * 2 + b]);
             }
-            umma_commit(&s_full[t * 2 + b]);
+            __syncwarp();
         };
         bool ok = true;
         if (most > 0) {
@@ -252,159 +275,145 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
                 ok = wait_all(&p_ready[t * 2 + b], parity, 54);
                 if (!ok) continue;
                 tcgen05_fence_after();
-                if (lane == 0) {
-                    const uint64_t vd = umma_desc_k_major_sw128(sV + b * S::kV);
+                if (elected) {
+                    const uint64_t vd = desc_k_major(av + b * S::kV);
 #pragma unroll
                     for (int k = 0; k < kN / 16; ++k)
-                        mma_ts(tmem + (uint32_t)(t * 256 + 2 * kN), tmem + (uint32_t)(t * 256 + b * kN + k * 8), vd + (uint64_t)(k * 32 >> 4), idesc(D), j > 0 || k != 0);
+                        mma_ts(tm + (uint32_t)(t * 256 + 2 * kN), tm + (uint32_t)(t * 256 + b * kN + k * 8), vd + (uint64_t)(k * 32 >> 4), idesc(D), j > 0 || k != 0);
                     umma_commit(&pv_done[t * 2 + b]);
                 }
                 __syncwarp();
             }
         }
     } else if (active && warp > kMmaWarp) {
-        // ---- taking the codes apart ----
-        const int take = warp - kMmaWarp - 1;
-        const int* table = block_table + (size_t)r * table_stride;
-        const int per_page = page_size / kBlock;
-        // keys: a warp has one of the tile's four blocks; lane = (token, quarter), tokens in the order 0 4 1 5 2 6 3 7 so that the 16-byte
-        // stores of eight lanes meet in no bank
-        const int quarter = lane & 3, token = ((lane >> 3) & 3) + ((lane >> 2) & 1) * 4;
-        // values: lane = (eight keys, eighth of a group); a warp has half of the eighths and half of the groups
-        const int octet = lane & 7, eighth = (take >> 1) * 4 + (lane >> 3), g0 = (take & 1) * HG;
-        auto lookup = [&](int j, int block) {
-            const int b = (k_lo + j * kN) / kBlock + block, index = b / per_page;
-            if (j >= most || b * kBlock >= seq_len || index >= table_stride) return -1;
-            const int page = __ldg(table + index);
-            return page >= 0 && page < num_pages ? (page * nkv + kvh) * per_page + (b - index * per_page) : -1;
+        // ---- taking the codes apart: warps 0-3 of these the keys (and asking for the blocks), 4-7 the values ----
+        const int take = (warp - kMmaWarp - 1) & 3;
+        const bool values = warp - kMmaWarp - 1 >= kTakeWarps;
+        unsigned char* raw = base + S::kRaw;
+        // a tile's buffer b is free when the last row tile that had tile j - 2 is through with it (one thread issues the MMAs in order)
+        auto free_again = [&](uint64_t* bars2, int j, int code) {
+            return j < 2 || wait_all(&bars2[(j - 2 < tiles[1] ? 2 : 0) + (j & 1)], (uint32_t)(((j >> 1) - 1) & 1), code);
         };
-        Words<NG> kc[2];
-        Words<HG> kw[2], vc[4], vw[4];
-        int id_k = lookup(0, take), id_v = lookup(0, octet >> 1);
-        bool none = false;
-        auto load = [&]() {
-            none = id_k < 0;
-            const unsigned char* kb = cache + (size_t)max(id_k, 0) * kBytes;
+        if (!values) {
+            const int* table = block_table + (size_t)r * table_stride;
+            const int per_page = page_size / kBlock;
+            // a warp has one of the tile's four blocks; lane = (token, quarter), tokens in the order 0 4 1 5 2 6 3 7 so that the 16-byte stores
+            // of eight lanes meet in no bank
+            const int quarter = lane & 3, token = ((lane >> 3) & 3) + ((lane >> 2) & 1) * 4;
+            auto lookup = [&](int j) {
+                const int b = (k_lo + j * kN) / kBlock + take, index = b / per_page;
+                if (j >= most || b * kBlock >= seq_len || index >= table_stride) return -1;
+                const int page = __ldg(table + index);
+                return page >= 0 && page < num_pages ? (page * nkv + kvh) * per_page + (b - index * per_page) : -1;
+            };
+            // what the table does not name is not copied
+            int ids = -1;                                           // lane l: this warp's block of tile 32 n + l
+            auto request = [&](int j) {
+                if ((j & 31) == 0) ids = lookup(j + lane);
+                if (j >= most || lane != (j & 31)) return;
+                const int stage = j % kRawStages;
+                if (ids < 0 && k_lo + j * kN + take * kBlock < seq_len) atomicOr(&s_missing[j & 7], 1 << take);
+                else atomicAnd(&s_missing[j & 7], ~(1 << take));
+                mbar_expect_tx(&raw_full[stage], ids >= 0 ? kBytes : 0);
+                if (ids >= 0) bulk_load(raw + (stage * (kN / kBlock) + take) * S::kRawBlock, cache + (size_t)ids * kBytes, kBytes, &raw_full[stage]);
+            };
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int t = token + 8 * h;
-                kc[h] = reinterpret_cast<const Words<NG>*>(kb)[t * 4 + quarter];
-                kw[h] = reinterpret_cast<const Words<HG>*>(kb + key_words_at(D))[t];
-            }
-            const unsigned char* vb = cache + (size_t)max(id_v, 0) * kBytes;
+            for (int i = 0; i < kRawStages - 1; ++i) request(i);
+            for (int j = 0; j < most; ++j) {
+                const int b = j & 1;
+                // the stage of tile j - 1 is refilled once all warps have read it
+                if (j > 0 && !wait_all(&raw_free[(j - 1) % kRawStages], (uint32_t)(((j - 1) / kRawStages) & 1), 64)) break;
+                request(j + kRawStages - 1);
+                __syncwarp();
+                if (!wait_all(&raw_full[j % kRawStages], (uint32_t)((j / kRawStages) & 1), 63)) break;
+                const unsigned char* kb = raw + ((j % kRawStages) * (kN / kBlock) + take) * S::kRawBlock;
+                if (!free_again(s_full, j, 55)) break;
+                unsigned char* kt = sK + b * S::kK;
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                vc[p] = reinterpret_cast<const Words<HG>*>(vb + value_codes_at(D))[(((octet & 1) * 8 + eighth) * 4 + p) * 2 + (take & 1)];
-                vw[p] = reinterpret_cast<const Words<HG>*>(vb + value_words_at(D))[((octet & 1) * 4 + p) * 2 + (take & 1)];
-                if (id_v < 0)
+                for (int h = 0; h < 2; ++h) {
+                    const int row = take * kBlock + token + 8 * h;
+                    const Words<NG> kc = reinterpret_cast<const Words<NG>*>(kb)[(token + 8 * h) * 4 + quarter];
+                    const Words<HG> kw = reinterpret_cast<const Words<HG>*>(kb + key_words_at(D))[token + 8 * h];
 #pragma unroll
-                    for (int k = 0; k < HG; ++k) vw[p].w[k] = 0;
-            }
-        };
-        auto note = [&](int b, int key, int j, unsigned group) {
-            unsigned old = *(volatile unsigned*)&s_bad[b][key], seen;
-            do {
-                seen = old;
-                old = atomicCAS(&s_bad[b][key], seen, (seen >> 8) == (unsigned)(j + 1) ? seen | group : ((unsigned)(j + 1) << 8) | group);
-            } while (old != seen);
-            atomicExch(&s_any[b], (unsigned)(j + 1));
-        };
-        if (most > 0) load();
-        for (int j = 0; j < most; ++j) {
-            const int b = j & 1;
-            const uint32_t parity = ((j >> 1) - 1) & 1;
-            const int key0 = k_lo + j * kN;
-            const bool missing = none && key0 + take * kBlock < seq_len;
-            id_k = lookup(j + 1, take), id_v = lookup(j + 1, octet >> 1);
-            // ---- keys ----
-            if (j >= 2) {
-                bool ok = true;
-                if (j - 2 < tiles[0]) ok = wait_all(&s_full[b], parity, 55);
-                if (ok && j - 2 < tiles[1]) ok = wait_all(&s_full[2 + b], parity, 56);
-                if (!ok) break;
-            }
-            unsigned char* kt = sK + b * S::kK;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int row = take * kBlock + token + 8 * h;
-#pragma unroll
-                for (int k = 0; k < NG; ++k) {
-                    const uint32_t w = k & 1 ? __byte_perm(kw[h].w[k >> 1], 0, 0x3232) : __byte_perm(kw[h].w[k >> 1], 0, 0x1010);
-                    const uint32_t zero = mul_bf16x2(w & 0x000f000fu, kMinus2p127), step = mul_bf16x2(w & 0xfff0fff0u, k64);
-                    const uint32_t x = kc[h].w[k], y = x >> 8;
-                    uint4 v;
-                    v.x = mul_bf16x2(fma_bf16x2(x & 0x000f000fu, k2p127, zero), step);
-                    v.y = mul_bf16x2(fma_bf16x2(x & 0x00f000f0u, k2p123, zero), step);
-                    v.z = mul_bf16x2(fma_bf16x2(y & 0x000f000fu, k2p127, zero), step);
-                    v.w = mul_bf16x2(fma_bf16x2(y & 0x00f000f0u, k2p123, zero), step);
-                    *reinterpret_cast<uint4*>(kt + (k >> 1) * (kN * 128) + row * 128 + ((((k & 1) * 4 + quarter) ^ (row & 7)) << 4)) = v;
+                    for (int k = 0; k < NG; ++k) {
+                        const uint32_t w = k & 1 ? __byte_perm(kw.w[k >> 1], 0, 0x3232) : __byte_perm(kw.w[k >> 1], 0, 0x1010);
+                        const uint32_t zero = mul_bf16x2(w & 0x000f000fu, kMinus2p127), step = mul_bf16x2(w & 0xfff0fff0u, k64);
+                        const uint32_t x = kc.w[k], y = x >> 8;
+                        uint4 v;
+                        v.x = mul_bf16x2(fma_bf16x2(x & 0x000f000fu, k2p127, zero), step);
+                        v.y = mul_bf16x2(fma_bf16x2(x & 0x00f000f0u, k2p123, zero), step);
+                        v.z = mul_bf16x2(fma_bf16x2(y & 0x000f000fu, k2p127, zero), step);
+                        v.w = mul_bf16x2(fma_bf16x2(y & 0x00f000f0u, k2p123, zero), step);
+                        *reinterpret_cast<uint4*>(kt + (k >> 1) * (kN * 128) + row * 128 + ((((k & 1) * 4 + quarter) ^ (row & 7)) << 4)) = v;
+                    }
                 }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&k_full[b]), mbar_arrive(&raw_free[j % kRawStages]);
             }
-            if (lane == 0) {
-                if (missing) atomicOr(&s_missing[j & 3], 1 << take);
-                else atomicAnd(&s_missing[j & 3], ~(1 << take));
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&k_full[b]);
-            // ---- values ----
-            if (j >= 2) {
-                bool ok = true;
-                if (j - 2 < tiles[0]) ok = wait_all(&pv_done[b], parity, 57);
-                if (ok && j - 2 < tiles[1]) ok = wait_all(&pv_done[2 + b], parity, 58);
-                if (!ok) break;
-            }
-            if (key0 + kN > seq_len) {                              // keys behind the last one: whatever lies there is no number
+        } else {
+            // lane = (eight keys, eighth of a group); a warp has half of the eighths and half of the groups
+            const int octet = lane & 7, eighth = (take >> 1) * 4 + (lane >> 3), g0 = (take & 1) * HG;
+            for (int j = 0; j < most; ++j) {
+                const int b = j & 1;
+                const int key0 = k_lo + j * kN;
+                if (!wait_all(&raw_full[j % kRawStages], (uint32_t)((j / kRawStages) & 1), 65)) break;
+                const unsigned char* vb = raw + ((j % kRawStages) * (kN / kBlock) + (octet >> 1)) * S::kRawBlock;
+                Words<HG> vc[4], vw[4];
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
-                    const int key = key0 + octet * 8 + 2 * p;
-                    const uint32_t keep = (key < seq_len ? 0xffffu : 0u) | (key + 1 < seq_len ? 0xffff0000u : 0u);
-#pragma unroll
-                    for (int k = 0; k < HG; ++k) vw[p].w[k] &= keep;
+                    vc[p] = reinterpret_cast<const Words<HG>*>(vb + value_codes_at(D))[(((octet & 1) * 8 + eighth) * 4 + p) * 2 + (take & 1)];
+                    vw[p] = reinterpret_cast<const Words<HG>*>(vb + value_words_at(D))[((octet & 1) * 4 + p) * 2 + (take & 1)];
                 }
-            }
-            uint32_t odd = 0;                                       // a sign bit is set where a word is not a number
+                const int missing = *(volatile int*)&s_missing[j & 7];
+                if (missing != 0 || key0 + kN > seq_len) {          // keys behind the last one and of no page: their weights are zero
 #pragma unroll
-            for (int p = 0; p < 4; ++p)
+                    for (int p = 0; p < 4; ++p) {
+                        const int key = key0 + octet * 8 + 2 * p;
+                        const uint32_t keep = (missing >> (octet >> 1)) & 1 ? 0u : (key < seq_len ? 0xffffu : 0u) | (key + 1 < seq_len ? 0xffff0000u : 0u);
 #pragma unroll
-                for (int k = 0; k < HG; ++k) odd |= (vw[p].w[k] & 0x7f807f80u) + 0x00800080u;
-            if (__any_sync(0xffffffffu, (odd & 0x80008000u) != 0)) {
+                        for (int k = 0; k < HG; ++k) vw[p].w[k] &= keep;
+                    }
+                }
+                uint32_t odd = 0;                                   // a sign bit is set where a word is not a number
+#pragma unroll
+                for (int p = 0; p < 4; ++p)
+#pragma unroll
+                    for (int k = 0; k < HG; ++k) odd |= (vw[p].w[k] & 0x7f807f80u) + 0x00800080u;
                 if (odd & 0x80008000u) {
+                    atomicExch(&s_odd, 1);
 #pragma unroll
                     for (int p = 0; p < 4; ++p)
 #pragma unroll
                         for (int k = 0; k < HG; ++k) {
                             const uint32_t at = ((vw[p].w[k] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-                            const int key = octet * 8 + 2 * p;
-                            if (at & 0x8000u) note(b, key, j, 1u << (g0 + k)), vw[p].w[k] &= 0xffff0000u;
-                            if (at & 0x80000000u) note(b, key + 1, j, 1u << (g0 + k)), vw[p].w[k] &= 0xffffu;
+                            vw[p].w[k] &= (at & 0x8000u ? 0u : 0xffffu) | (at & 0x80000000u ? 0u : 0xffff0000u);
                         }
                 }
+                if (!free_again(pv_done, j, 57)) break;
+                unsigned char* vt = sV + b * S::kV;
+#pragma unroll
+                for (int k = 0; k < HG; ++k) {
+                    uint32_t v[4][4];                               // [column][pair of keys]
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        const uint32_t w = vw[p].w[k], zero = mul_bf16x2(w & 0x000f000fu, kMinus2p127), step = mul_bf16x2(w & 0xfff0fff0u, k64);
+                        const uint32_t x = vc[p].w[k], y = x >> 8;
+                        v[0][p] = mul_bf16x2(fma_bf16x2(x & 0x000f000fu, k2p127, zero), step);
+                        v[1][p] = mul_bf16x2(fma_bf16x2(x & 0x00f000f0u, k2p123, zero), step);
+                        v[2][p] = mul_bf16x2(fma_bf16x2(y & 0x000f000fu, k2p127, zero), step);
+                        v[3][p] = mul_bf16x2(fma_bf16x2(y & 0x00f000f0u, k2p123, zero), step);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = (g0 + k) * kGroup + eighth * 4 + i;
+                        *reinterpret_cast<uint4*>(vt + row * 128 + ((octet ^ (row & 7)) << 4)) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
+                if (lane == 0) mbar_arrive(&v_full[b]), mbar_arrive(&raw_free[j % kRawStages]);
             }
-            unsigned char* vt = sV + b * S::kV;
-#pragma unroll
-            for (int k = 0; k < HG; ++k) {
-                uint32_t v[4][4];                                   // [column][pair of keys]
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    const uint32_t w = vw[p].w[k], zero = mul_bf16x2(w & 0x000f000fu, kMinus2p127), step = mul_bf16x2(w & 0xfff0fff0u, k64);
-                    const uint32_t x = vc[p].w[k], y = x >> 8;
-                    v[0][p] = mul_bf16x2(fma_bf16x2(x & 0x000f000fu, k2p127, zero), step);
-                    v[1][p] = mul_bf16x2(fma_bf16x2(x & 0x00f000f0u, k2p123, zero), step);
-                    v[2][p] = mul_bf16x2(fma_bf16x2(y & 0x000f000fu, k2p127, zero), step);
-                    v[3][p] = mul_bf16x2(fma_bf16x2(y & 0x00f000f0u, k2p123, zero), step);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = (g0 + k) * kGroup + eighth * 4 + i;
-                    *reinterpret_cast<uint4*>(vt + row * 128 + ((octet ^ (row & 7)) << 4)) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&v_full[b]);
-            if (j + 1 < most) load();
         }
     } else if (active && warp < kSoftWarps) {
         // ---- softmax: a thread per row (TMEM lane 32 * (warp % 4) + lane) ----
@@ -416,7 +425,6 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
         const int pos = row_ok ? seq_len - n + grow / g : -1;
         const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(t * 256), o_addr = lane_addr + 2 * kN;
         float m_used = -INFINITY, l = 0.f;
-        unsigned bad = 0;                               // groups whose sum holds a value that is not a number
         bool ok = true;
         for (int j = 0; j < my_tiles; ++j) {
             const int b = j & 1;
@@ -424,7 +432,7 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             ok = wait_all(&s_full[t * 2 + b], (uint32_t)((j >> 1) & 1), 59);
             if (!ok) break;
             tcgen05_fence_after();
-            const int missing = *(volatile int*)&s_missing[j & 3];
+            const int missing = *(volatile int*)&s_missing[j & 7];
             const bool need_mask = key0 + kN - 1 > pos || window > 0 || missing != 0;
             const int hi = pos - key0;                              // columns <= hi are visible ...
             const int lo = window > 0 ? hi - window : -1;           // ... and > lo
@@ -481,16 +489,6 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             }
             tst32(lane_addr + (uint32_t)(b * kN), p);
             tst_wait();
-            // values that are not numbers are noted when their tile is complete, and a buffer's notes are good until its next P V is done
-            // (this row's own P has to arrive for that)
-            ok = wait_all(&v_full[b], (uint32_t)((j >> 1) & 1), 61);
-            if (!ok) break;
-            if (*(volatile unsigned*)&s_any[b] == (unsigned)(j + 1)) {
-                for (int e = 0; e < kN; ++e) {
-                    const unsigned what = *(volatile unsigned*)&s_bad[b][e];
-                    if (e <= hi && e > lo && !((missing >> (e / kBlock)) & 1) && (what >> 8) == (unsigned)(j + 1)) bad |= what & 255u;
-                }
-            }
             tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_ready[t * 2 + b]);
@@ -502,6 +500,18 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
         constexpr int kPieces = D / 8;                              // 16-byte pieces of a row
         if (*(volatile int*)&s_abort == 0 && has[t]) {
             const float f = l == 0.f ? 0.f : __fdividef(1.f, l);
+            unsigned bad = 0;                           // groups whose sum holds a value that is not a number
+            if (*(volatile int*)&s_odd && row_ok) {
+                const int* table = block_table + (size_t)r * table_stride;
+                for (int key = window > 0 ? max(0, pos - window + 1) : 0; key <= pos && key / page_size < table_stride; ++key) {
+                    const int page = table[key / page_size];
+                    if (page < 0 || page >= num_pages) continue;
+                    const unsigned char* block = cache + ((size_t)(page * nkv + kvh) * (page_size / kBlock) + key % page_size / kBlock) * kBytes;
+                    const uint16_t* words = reinterpret_cast<const uint16_t*>(block + value_words_at(D)) + ((key % kBlock) >> 1) * NG * 2 + (key & 1);
+                    for (int k = 0; k < NG; ++k)
+                        if ((words[2 * k] & 0x7f80u) == 0x7f80u) bad |= 1u << k;
+                }
+            }
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
