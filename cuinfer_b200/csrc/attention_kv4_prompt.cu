@@ -10,7 +10,7 @@
 //   * S = Q K^T and O += P V are `tcgen05.mma.cta_group::1.kind::f16`, S, P and O in tensor memory (2 x (64 + 64 + 128) columns), issued by one
 //     thread; S of key tile j + 1 is computed while the softmax warps take the exponentials of tile j.
 //   * Eight softmax warps, a thread per row: running maximum in base 2 that is raised when it grows by more than 8 (or at all over the
-//     first 256 keys), the sum is of the rounded weights; P goes back over its scores in bfloat16.
+//     first 256 keys); P goes back over its scores in bfloat16, which rounds each weight once (2^-9 of it), the sum is of the weights before that.
 //   * Rows see the keys up to their position, the last `window` of them, and none of a page that the block table does not name.  A value that is not
 //     a number must not reach rows that do not see its key (0 x NaN is NaN): it is written as zero, and where a CTA has met one, its rows look
 //     through the words of the values that they see at the end.
@@ -79,6 +79,32 @@ __device__ __forceinline__ void tst32(uint32_t taddr, const uint32_t (&r)[32]) {
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(tc_smem_u32(dst)), "l"(src), "r"(bytes), "r"(tc_smem_u32(bar)) : "memory");
+}
+// two 32-bit numbers at a time
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 __device__ __forceinline__ void tst_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -447,7 +473,8 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             }
             float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < kN; ++e) part[e & 3] = fmaxf(part[e & 3], __uint_as_float(v[e / 32][e % 32]));
+            for (int e = 0; e < kN; e += 2)
+                part[(e >> 1) & 3] = max3(part[(e >> 1) & 3], __uint_as_float(v[e / 32][e % 32]), __uint_as_float(v[e / 32][e % 32 + 1]));
             const float mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * scale_log2;
             float corr = 1.f;
             bool rescale = false;
@@ -458,21 +485,21 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
                 rescale = j > 0;
             }
             const float m_eff = m_used == -INFINITY ? 0.f : m_used;
+            // P = 2^(s * scale - m), two at a time: a packed multiply-add, two ex2, a packed addition and a conversion
+            const uint64_t scale2 = pack2(scale_log2, scale_log2), minus_m = pack2(-m_eff, -m_eff);
             uint32_t p[32];
-            float sums[2] = {0.f, 0.f};
+            uint64_t sums[2] = {0, 0};
 #pragma unroll
             for (int e = 0; e < kN; e += 2) {
-                float pe[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const float x = fmaf(__uint_as_float(v[e / 32][e % 32 + u]), scale_log2, -m_eff);
-                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(pe[u]) : "f"(x));
-                }
-                p[e / 2] = pack_bf16(pe[0], pe[1]);
-                sums[0] += __uint_as_float(p[e / 2] << 16);
-                sums[1] += __uint_as_float(p[e / 2] & 0xffff0000u);
+                const float2 x = unpack2(fma2(pack2(__uint_as_float(v[e / 32][e % 32]), __uint_as_float(v[e / 32][e % 32 + 1])), scale2, minus_m));
+                float2 y;
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(x.x));
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(x.y));
+                sums[(e >> 1) & 1] = add2(sums[(e >> 1) & 1], pack2(y.x, y.y));
+                p[e / 2] = pack_bf16(y.x, y.y);
             }
-            l += sums[0] + sums[1];
+            const float2 sum = unpack2(add2(sums[0], sums[1]));
+            l += sum.x + sum.y;
             if (j > 0 && __any_sync(0xffffffffu, rescale)) {
                 ok = wait_all(&pv_done[t * 2 + (b ^ 1)], (uint32_t)(((j - 1) >> 1) & 1), 60);
                 if (!ok) break;

@@ -51,22 +51,31 @@ __device__ __forceinline__ unsigned char* block_of(unsigned char* cache, int slo
     return cache + (((size_t)page * nkv + kvh) * (page_size / kBlock) + block) * (size_t)block_bytes(d);
 }
 
+// x / s rounded to nearest, from r = 1 / s rounded to nearest: the quotient's remainder is exact in a fused multiply-add, and adding it times r
+// rounds correctly (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", IBM J. Res. Dev. 34, 1990).
+// Where it underflows, |x| is far below a step and the code does not depend on it.
+__device__ __forceinline__ float quotient(float x, float s, float r) {
+    const float q = __fmul_rn(x, r);
+    return __fmaf_rn(__fmaf_rn(-q, s, x), r, q);
+}
+
 struct Scale {
-    float step, zero;
+    float step, inverse, zero;
     uint32_t word;
 };
 
 // lo <= 0 <= hi; `bad`: a value of the group is not finite or too large
 __device__ __forceinline__ Scale scale_of(float lo, float hi, bool bad) {
     Scale s;
-    const float t = fmaxf(__fdiv_rn(__fsub_rn(hi, lo), 15.f), 7.5231638452626401e-37f);      // 2^-120
+    const float t = fmaxf(quotient(__fsub_rn(hi, lo), 15.f, 1.f / 15.f), 7.5231638452626401e-37f);      // 2^-120
     s.step = __uint_as_float((__float_as_uint(t) + 0xfffffu) & ~0xfffffu);
-    s.zero = rintf(__fdiv_rn(-lo, s.step));
+    s.inverse = __frcp_rn(s.step);
+    s.zero = rintf(quotient(-lo, s.step, s.inverse));
     s.word = bad ? kNanWord : (__float_as_uint(s.step) >> 16) | (uint32_t)s.zero;
     return s;
 }
 __device__ __forceinline__ uint32_t code_of(float x, const Scale& s, bool bad) {
-    return bad ? 0u : (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x, s.step)) + s.zero, 0.f), 15.f);
+    return bad ? 0u : (uint32_t)fminf(fmaxf(rintf(quotient(x, s.step, s.inverse)) + s.zero, 0.f), 15.f);
 }
 // (false for NaN)
 __device__ __forceinline__ bool holds(float x) { return fabsf(x) < 1.7014118346046923e38f; }     // 2^127

@@ -113,6 +113,248 @@ write_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, const int* __
     }
 }
 
+template <typename T, int E>
+struct alignas(sizeof(T) * E > 16 ? 16 : sizeof(T) * E) Lane {
+    T v[E];
+};
+
+// Head sizes 64, 128 and 256 with a rotation whose halves are whole lanes (the common cases).  A lane has E = D / 32 neighbouring values of a
+// head, 32 / E lanes a group; a warp takes HB heads of one token: all their loads are issued at once, and what depends on the token only
+// (slot, position, table row, gains) is fetched once and before the wait for the kernel in front.  The rotation's partner
+// lies `rotary / 2 / E` lanes away; it is exchanged as it came, so that the exchange is exact, and normed again where it arrives.
+// Bound by the memory's latency at few tokens; at many by instructions: a key head costs about four times a query head (64-bit norm
+// and rotation, quantisation).
+template <typename T, int E, int HB>
+__global__ void __launch_bounds__(kWarps * 32)
+write_lanes_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, const int* __restrict__ positions, const int* __restrict__ slots, AnyVec q_gain,
+                   AnyVec k_gain, int has_norm, float eps, const float* __restrict__ rope_table, int rotary, int max_positions,
+                   unsigned char* __restrict__ cache, int num_pages, int page_size, int nq, int nkv, int num_tokens) {
+    constexpr int D = 32 * E, NG = E, kLanes = 32 / E;               // lanes of a group
+    const int lane = threadIdx.x & 31;
+    const int heads = nq + 2 * nkv, chunks = (heads + HB - 1) / HB;
+    const int w = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int t = w / chunks, base = (w - t * chunks) * HB;
+    const bool live = t < num_tokens;
+    const int i0 = lane * E;
+    const int reach = rotary / (2 * E);                              // lanes of half a rotation
+    const bool rotates = lane < 2 * reach;
+    const int partner = !rotates ? lane : lane < reach ? lane + reach : lane - reach;
+    int slot = -1;
+    float cs[2 * E], gain_q[E], gain_k[E], gain_p[E];                // cosines and sines; gains of this lane and, for keys, of its partner
+    if (live) {
+        slot = slots[t];
+        if (rotates) {
+            int pos = positions[t];
+            pos = pos < 0 ? 0 : (pos >= max_positions ? max_positions - 1 : pos);
+            const float* tp = rope_table + (size_t)pos * rotary + 2 * ((lane < reach ? lane : lane - reach) * E);
+#pragma unroll
+            for (int e = 0; e < 2 * E; e += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(tp + e);
+                cs[e] = v.x, cs[e + 1] = v.y, cs[e + 2] = v.z, cs[e + 3] = v.w;
+            }
+        }
+        if (has_norm) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if (base < nq) gain_q[e] = q_gain[i0 + e];
+                if (base + HB > nq) gain_k[e] = k_gain[i0 + e], gain_p[e] = k_gain[partner * E + e];
+            }
+        }
+    }
+    griddep_wait();
+    griddep_launch();
+    if (!live) return;
+    const T* src = qkv + (size_t)t * row_stride + (size_t)base * D + i0;
+    Lane<T, E> raw[HB];
+#pragma unroll
+    for (int h = 0; h < HB; ++h)
+        if (base + h < heads) raw[h] = *reinterpret_cast<const Lane<T, E>*>(src + h * D);
+    unsigned char* block0 = block_of(cache, slot, num_pages, page_size, nkv, 0, D);
+    const size_t head_bytes = (size_t)(page_size / kBlock) * block_bytes(D);
+    const int token = block0 == nullptr ? 0 : slot % page_size % kBlock;
+#pragma unroll
+    for (int h = 0; h < HB; ++h) {
+        const int head = base + h;
+        if (head >= heads) break;
+        const int kind = head < nq ? 0 : (head < nq + nkv ? 1 : 2);
+        float x[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = to_f32(raw[h].v[e]);
+        if (kind == 0) {
+            if (has_norm) {
+                float ss = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) ss += x[e] * x[e];
+                const float factor = rsqrtf(warp_sum(ss) / (float)D + eps);
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = x[e] * factor * gain_q[e];
+            }
+            if (reach > 0) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float other = __shfl_sync(0xffffffffu, x[e], partner);
+                    if (rotates) x[e] = lane < reach ? x[e] * cs[2 * e] - other * cs[2 * e + 1] : x[e] * cs[2 * e] + other * cs[2 * e + 1];
+                }
+            }
+            Lane<T, E> o;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o.v[e] = from_f32<T>(x[e]);
+            *reinterpret_cast<Lane<T, E>*>(q_out + (size_t)t * q_stride + (size_t)head * D + i0) = o;
+            continue;
+        }
+        if (block0 == nullptr) continue;
+        unsigned char* block = block0 + (head - nq - (kind == 2 ? nkv : 0)) * head_bytes;
+        if (kind == 1 && (has_norm || reach > 0)) {
+            double factor = 1.0;
+            if (has_norm) {
+                double ss = 0.0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) ss += (double)x[e] * (double)x[e];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                factor = 1.0 / sqrt(ss / (double)D + (double)eps);
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float other = __shfl_sync(0xffffffffu, x[e], partner);
+                double a = has_norm ? (double)x[e] * factor * (double)gain_k[e] : (double)x[e];
+                if (rotates) {
+                    const double b = has_norm ? (double)other * factor * (double)gain_p[e] : (double)other;
+                    const double c = cs[2 * e], s = cs[2 * e + 1];
+                    a = lane < reach ? a * c - b * s : a * c + b * s;
+                }
+                // (the exchange of value e is over before x[e] changes: all lanes are here)
+                x[e] = (float)a;
+            }
+        }
+        float lo = 0.f, hi = 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < E; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]), bad = bad || !holds(x[e]);
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        const uint32_t group_lanes = (kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1u) << (lane / kLanes * kLanes));
+        bad = (__ballot_sync(0xffffffffu, bad) & group_lanes) != 0;
+        const Scale s = scale_of(lo, hi, bad);
+        uint32_t code[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) code[e] = code_of(x[e], s, bad);
+        const int g = lane / kLanes, in = (lane & (kLanes - 1)) * E;   // this lane's first value within its group
+        if (kind == 1) {
+            // eight values a word, value e of them in bits 4 (e / 2) + 16 (e % 2)
+            uint32_t word = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int at = (in + e) & 7;
+                word |= code[e] << (4 * (at >> 1) + 16 * (at & 1));
+            }
+#pragma unroll
+            for (int o = 1; o < 8 / E; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
+            if ((in & 7) == 0) reinterpret_cast<uint32_t*>(block)[(token * 4 + (in >> 3)) * NG + g] = word;
+            if (in == 0) reinterpret_cast<uint16_t*>(block + key_words_at(D))[token * NG + g] = (uint16_t)s.word;
+        } else {
+            // four values a half word
+            constexpr int kHalves = E > 4 ? E / 4 : 1;
+            uint16_t* codes = reinterpret_cast<uint16_t*>(block + value_codes_at(D));
+#pragma unroll
+            for (int u = 0; u < kHalves; ++u) {
+                uint32_t half = 0;
+#pragma unroll
+                for (int e = 0; e < (E > 4 ? 4 : E); ++e) half |= code[4 * u + e] << (4 * ((in + e) & 3));
+                if (E == 2) half |= __shfl_xor_sync(0xffffffffu, half, 1);
+                const int word = (((token >> 3) * 8 + (in >> 2) + u) * 4 + ((token & 7) >> 1)) * NG + g;
+                if (E >= 4 || (in & 3) == 0) codes[word * 2 + (token & 1)] = (uint16_t)half;
+            }
+            if (in == 0) reinterpret_cast<uint16_t*>(block + value_words_at(D))[((token >> 1) * NG + g) * 2 + (token & 1)] = (uint16_t)s.word;
+        }
+    }
+}
+
+// A warp per (slot, HB kv heads), a lane E = D / 32 neighbouring values: head sizes 64, 128 and 256.
+template <typename T, int E, int HB>
+__global__ void __launch_bounds__(kWarps * 32)
+read_lanes_kernel(unsigned char* __restrict__ cache, int num_pages, int page_size, const int* __restrict__ slots, T* __restrict__ keys, int key_stride,
+                  T* __restrict__ values, int value_stride, int nkv, int num_slots) {
+    constexpr int D = 32 * E, NG = E, kLanes = 32 / E;
+    const int lane = threadIdx.x & 31;
+    const int chunks = (nkv + HB - 1) / HB;
+    const int w = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int t = w / chunks, base = (w - t * chunks) * HB;
+    griddep_wait();
+    griddep_launch();
+    if (t >= num_slots) return;
+    const int slot = slots[t];
+    const unsigned char* block0 = block_of(cache, slot, num_pages, page_size, nkv, base, D);
+    if (block0 == nullptr) return;
+    const size_t head_bytes = (size_t)(page_size / kBlock) * block_bytes(D);
+    const int token = slot % page_size % kBlock;
+    const int g = lane / kLanes, in = (lane & (kLanes - 1)) * E;
+    uint32_t kc[HB], kw[HB], vw[HB], vc[HB];
+#pragma unroll
+    for (int h = 0; h < HB; ++h) {
+        if (base + h >= nkv) break;
+        const unsigned char* block = block0 + h * head_bytes;
+        kc[h] = reinterpret_cast<const uint32_t*>(block)[(token * 4 + (in >> 3)) * NG + g];
+        kw[h] = reinterpret_cast<const uint16_t*>(block + key_words_at(D))[token * NG + g];
+        vw[h] = reinterpret_cast<const uint16_t*>(block + value_words_at(D))[((token >> 1) * NG + g) * 2 + (token & 1)];
+        const uint16_t* codes = reinterpret_cast<const uint16_t*>(block + value_codes_at(D));
+        const int word = (((token >> 3) * 8 + (in >> 2)) * 4 + ((token & 7) >> 1)) * NG + g;
+        vc[h] = codes[word * 2 + (token & 1)];
+        if (E == 8) vc[h] |= (uint32_t)codes[(word + 4 * NG) * 2 + (token & 1)] << 16;
+    }
+#pragma unroll
+    for (int h = 0; h < HB; ++h) {
+        if (base + h >= nkv) break;
+        Lane<T, E> k, v;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int at = (in + e) & 7;
+            k.v[e] = from_f32<T>(step_of(kw[h]) * (float)((int)((kc[h] >> (4 * (at >> 1) + 16 * (at & 1))) & 15u) - (int)(kw[h] & 15u)));
+            v.v[e] = from_f32<T>(step_of(vw[h]) * (float)((int)((vc[h] >> (4 * (E == 2 ? (in + e) & 3 : e))) & 15u) - (int)(vw[h] & 15u)));
+        }
+        *reinterpret_cast<Lane<T, E>*>(keys + (size_t)t * key_stride + (size_t)(base + h) * D + lane * E) = k;
+        *reinterpret_cast<Lane<T, E>*>(values + (size_t)t * value_stride + (size_t)(base + h) * D + lane * E) = v;
+    }
+}
+
+// From so many warps of a head each on, a warp takes four heads: the GPU is full either way.
+constexpr long long kManyHeads = 148 * 64;
+
+template <typename T>
+static cudaError_t launch_write(int d, cudaStream_t stream, bool use_pdl, const T* qkv, int row_stride, T* q_out, int q_stride, const int* positions, const int* slots,
+                                AnyVec qg, AnyVec kg, int has_norm, float eps, const float* rope_table, int rotary, int max_positions, unsigned char* cache,
+                                int num_pages, int page_size, int nq, int nkv, int num_tokens) {
+    const int heads = nq + 2 * nkv;
+    const bool many = (long long)num_tokens * heads >= kManyHeads;
+    const long long warps = (long long)num_tokens * ((heads + (many ? 3 : 0)) / (many ? 4 : 1));
+    const dim3 grid((unsigned)((warps + kWarps - 1) / kWarps));
+#define CIB_KV4_WRITE(EV, HB)                                                                                                                      \
+    return launch_pdl(write_lanes_kernel<T, EV, HB>, grid, dim3(kWarps * 32), 0, stream, use_pdl, qkv, row_stride, q_out, q_stride, positions, slots, qg, \
+                      kg, has_norm, eps, rope_table, rotary, max_positions, cache, num_pages, page_size, nq, nkv, num_tokens)
+    if (d == 64) { if (many) CIB_KV4_WRITE(2, 4); else CIB_KV4_WRITE(2, 1); }
+    if (d == 128) { if (many) CIB_KV4_WRITE(4, 4); else CIB_KV4_WRITE(4, 1); }
+    if (many) CIB_KV4_WRITE(8, 4); else CIB_KV4_WRITE(8, 1);
+#undef CIB_KV4_WRITE
+}
+
+template <typename T>
+static cudaError_t launch_read(int d, cudaStream_t stream, bool use_pdl, unsigned char* cache, int num_pages, int page_size, const int* slots, T* keys,
+                               int key_stride, T* values, int value_stride, int nkv, int num_slots) {
+    const bool many = (long long)num_slots * nkv >= kManyHeads;
+    const long long warps = (long long)num_slots * ((nkv + (many ? 3 : 0)) / (many ? 4 : 1));
+    const dim3 grid((unsigned)((warps + kWarps - 1) / kWarps));
+#define CIB_KV4_READ(EV, HB)                                                                                                                      \
+    return launch_pdl(read_lanes_kernel<T, EV, HB>, grid, dim3(kWarps * 32), 0, stream, use_pdl, cache, num_pages, page_size, slots, keys, key_stride,  \
+                      values, value_stride, nkv, num_slots)
+    if (d == 64) { if (many) CIB_KV4_READ(2, 4); else CIB_KV4_READ(2, 1); }
+    if (d == 128) { if (many) CIB_KV4_READ(4, 4); else CIB_KV4_READ(4, 1); }
+    if (many) CIB_KV4_READ(8, 4); else CIB_KV4_READ(8, 1);
+#undef CIB_KV4_READ
+}
+
 // A warp per (slot, kv head): rows of slots that are none are left as they are.
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32)
@@ -167,7 +409,17 @@ extern "C" int cib_qk_norm_rope_kv4_write(const void* qkv, int dtype, int row_st
     CIB_REQUIRE((heads + kv4::kWarps - 1) / kv4::kWarps <= 65535, "qk_norm_rope_kv4_write: %d heads are too many", heads);
     const dim3 grid(num_tokens, (heads + kv4::kWarps - 1) / kv4::kWarps);
     cudaError_t e;
-    if (dtype == kF32)
+    const int width = dtype == kF32 ? 4 : 2, lane_bytes = d / 32 * width < 16 ? d / 32 * width : 16;
+    const bool lanes = (d == 64 || d == 128 || d == 256) && rotary % (d / 16) == 0 && (uintptr_t)rope_table % 16 == 0 && (uintptr_t)qkv % lane_bytes == 0 &&
+                       (uintptr_t)q_out % lane_bytes == 0 && (size_t)row_stride * width % lane_bytes == 0 && (size_t)q_stride * width % lane_bytes == 0 &&
+                       (long long)num_tokens * heads < (1ll << 31);
+    if (lanes && dtype == kF32)
+        e = kv4::launch_write<float>(d, stream, use_pdl != 0, (const float*)qkv, row_stride, (float*)q_out, q_stride, positions, slots, qg, kg, has_norm, eps, rope_table,
+                                     rotary, max_positions, (unsigned char*)cache, num_pages, page_size, nq, nkv, num_tokens);
+    else if (lanes)
+        e = kv4::launch_write<__nv_bfloat16>(d, stream, use_pdl != 0, (const __nv_bfloat16*)qkv, row_stride, (__nv_bfloat16*)q_out, q_stride, positions, slots, qg, kg,
+                                             has_norm, eps, rope_table, rotary, max_positions, (unsigned char*)cache, num_pages, page_size, nq, nkv, num_tokens);
+    else if (dtype == kF32)
         e = launch_pdl(kv4::write_kernel<float>, grid, dim3(kv4::kWarps * 32), 0, stream, use_pdl != 0, (const float*)qkv, row_stride, (float*)q_out, q_stride,
                        positions, slots, qg, kg, has_norm, eps, rope_table, rotary, max_positions, (unsigned char*)cache, num_pages, page_size, nq, nkv, d);
     else
@@ -188,7 +440,16 @@ extern "C" int cib_kv4_read(const void* cache, int num_pages, int page_size, con
     if (num_slots == 0) return 0;
     const dim3 grid(num_slots, (nkv + kv4::kWarps - 1) / kv4::kWarps);
     cudaError_t e;
-    if (dtype == kF32)
+    const int width = dtype == kF32 ? 4 : 2, lane_bytes = d / 32 * width < 16 ? d / 32 * width : 16;
+    const bool lanes = (d == 64 || d == 128 || d == 256) && (uintptr_t)keys % lane_bytes == 0 && (uintptr_t)values % lane_bytes == 0 &&
+                       (size_t)key_stride * width % lane_bytes == 0 && (size_t)value_stride * width % lane_bytes == 0 && (long long)num_slots * nkv < (1ll << 31);
+    if (lanes && dtype == kF32)
+        e = kv4::launch_read<float>(d, stream, use_pdl != 0, (unsigned char*)cache, num_pages, page_size, slots, (float*)keys, key_stride, (float*)values, value_stride,
+                                    nkv, num_slots);
+    else if (lanes)
+        e = kv4::launch_read<__nv_bfloat16>(d, stream, use_pdl != 0, (unsigned char*)cache, num_pages, page_size, slots, (__nv_bfloat16*)keys, key_stride,
+                                            (__nv_bfloat16*)values, value_stride, nkv, num_slots);
+    else if (dtype == kF32)
         e = launch_pdl(kv4::read_kernel<float>, grid, dim3(kv4::kWarps * 32), 0, stream, use_pdl != 0, (unsigned char*)cache, num_pages, page_size, slots,
                        (float*)keys, key_stride, (float*)values, value_stride, nkv, d);
     else
