@@ -118,12 +118,216 @@ struct alignas(sizeof(T) * E > 16 ? 16 : sizeof(T) * E) Lane {
     T v[E];
 };
 
-// Head sizes 64, 128 and 256 with a rotation whose halves are whole lanes (the common cases).  A lane has E = D / 32 neighbouring values of a
+// Prompts: head sizes 64, 128 and 256, a rotation of the whole head or none.  A head lies in L = D / 16 lanes; a lane has eight values of its first
+// half and their rotation partners of the second, so nothing is exchanged but the sums; eight values are a whole word of key codes and two half
+// words of value codes.  A warp takes PASSES x 32 / L heads of one token, with all loads on their way at once.
+//
+// Keys are computed in 32 bits here too, together with a bound of their error, and only a warp that has a value (or a step) within
+// that bound of a border between two codes does it again in 64 bits: the codes are those of the 64-bit computation, which alone took
+// two thirds of the time.  The bound: the sum of squares is 8 + 8 additions deep at most (2^-21 of its root), the reciprocal root is good to 2
+// units (2^-22), two products, and the rotation's two products and sum: less than 2^-20.5 of |a cos| + |b sin| (2^-22.5 without a norm).
+constexpr int kRowWarps = 8;
+
+template <typename T>
+struct alignas(sizeof(T) * 8 > 16 ? 16 : sizeof(T) * 8) Eight {
+    T v[8];
+};
+
+template <typename T, int L, int PASSES>
+__global__ void __launch_bounds__(kRowWarps * 32)
+write_rows_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, const int* __restrict__ positions, const int* __restrict__ slots, AnyVec q_gain,
+                  AnyVec k_gain, int has_norm, float eps, const float* __restrict__ rope_table, int has_rope, int max_positions,
+                  unsigned char* __restrict__ cache, int num_pages, int page_size, int nq, int nkv, int num_tokens) {
+    constexpr int D = 16 * L, NG = D / kGroup, HPP = 32 / L;         // heads a pass
+    __shared__ __align__(16) float s_gain[2][D];
+    if (has_norm)
+        for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) s_gain[i / D][i % D] = i < D ? q_gain[i] : k_gain[i - D];
+    const int lane = threadIdx.x & 31, sub = lane / L, li = lane % L;
+    const int heads = nq + 2 * nkv, chunks = (heads + HPP * PASSES - 1) / (HPP * PASSES);
+    const int w = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+    const int t = w / chunks, base = (w - t * chunks) * HPP * PASSES;
+    const bool live = t < num_tokens;
+    float cs[16];
+    int slot = -1;
+    if (live) {
+        slot = slots[t];
+        if (has_rope) {
+            int pos = positions[t];
+            pos = pos < 0 ? 0 : (pos >= max_positions ? max_positions - 1 : pos);
+            const float4* tp = reinterpret_cast<const float4*>(rope_table + (size_t)pos * D + 16 * li);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float4 v = tp[e];
+                cs[4 * e] = v.x, cs[4 * e + 1] = v.y, cs[4 * e + 2] = v.z, cs[4 * e + 3] = v.w;
+            }
+        }
+    }
+    griddep_wait();
+    griddep_launch();
+    __syncthreads();
+    if (!live) return;
+    const T* src = qkv + (size_t)t * row_stride + 8 * li;
+    Eight<T> first[PASSES], second[PASSES];
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+        const int head = base + p * HPP + sub;
+        if (head < heads) {
+            first[p] = *reinterpret_cast<const Eight<T>*>(src + (size_t)head * D);
+            second[p] = *reinterpret_cast<const Eight<T>*>(src + (size_t)head * D + D / 2);
+        }
+    }
+    unsigned char* block0 = block_of(cache, slot, num_pages, page_size, nkv, 0, D);
+    const size_t head_bytes = (size_t)(page_size / kBlock) * block_bytes(D);
+    const int token = block0 == nullptr ? 0 : slot % page_size % kBlock;
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+        const int head = base + p * HPP + sub;
+        const int kind = head < nq ? 0 : (head < nq + nkv ? 1 : 2);          // (a head behind the last one: a value that is not stored)
+        const bool stored = head < heads;
+        if (base + p * HPP >= heads) break;
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = stored ? to_f32(first[p].v[e]) : 0.f, x[8 + e] = stored ? to_f32(second[p].v[e]) : 0.f;
+        float error = 0.f;                                           // of the values as they are computed below, at most
+        if (__any_sync(0xffffffffu, kind != 2)) {
+            if (has_norm) {
+                float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s0 = fmaf(x[e], x[e], s0), s1 = fmaf(x[8 + e], x[8 + e], s1);
+                float ss = s0 + s1;
+#pragma unroll
+                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const float factor = kind == 2 ? 1.f : rsqrtf(ss / (float)D + eps);
+                const float* gain = s_gain[kind == 0 ? 0 : 1] + 8 * li;
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    const float4 a = *reinterpret_cast<const float4*>(gain + e), b = *reinterpret_cast<const float4*>(gain + D / 2 + e);
+                    if (kind != 2) {
+                        x[e] = x[e] * factor * a.x, x[e + 1] = x[e + 1] * factor * a.y, x[e + 2] = x[e + 2] * factor * a.z, x[e + 3] = x[e + 3] * factor * a.w;
+                        x[8 + e] = x[8 + e] * factor * b.x, x[9 + e] = x[9 + e] * factor * b.y, x[10 + e] = x[10 + e] * factor * b.z, x[11 + e] = x[11 + e] * factor * b.w;
+                    }
+                }
+            }
+            if (kind != 2) {
+                if (has_rope) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float c = cs[2 * e], s = cs[2 * e + 1], a = x[e], b = x[8 + e];
+                        const float ac = a * c, bs = b * s, bc = b * c, as = a * s;
+                        x[e] = ac - bs;
+                        x[8 + e] = bc + as;
+                        if (kind == 1) error = fmaxf(error, fmaxf(fabsf(ac) + fabsf(bs), fabsf(bc) + fabsf(as)));
+                    }
+                } else if (kind == 1 && has_norm) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) error = fmaxf(error, fabsf(x[e]));
+                }
+                error *= has_norm ? 6.7434958e-07f : 1.6858740e-07f;       // 2^-20.5, 2^-22.5
+            }
+        }
+        if (kind == 0 && stored) {
+            Eight<T> a, b;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) a.v[e] = from_f32<T>(x[e]), b.v[e] = from_f32<T>(x[8 + e]);
+            T* dst = q_out + (size_t)t * q_stride + (size_t)head * D + 8 * li;
+            *reinterpret_cast<Eight<T>*>(dst) = a;
+            *reinterpret_cast<Eight<T>*>(dst + D / 2) = b;
+        }
+        if (block0 == nullptr || !__any_sync(0xffffffffu, kind != 0)) continue;
+        // ---- quantisation: groups are four lanes of either half ----
+        Scale scale[2];
+        bool bad[2];
+        uint32_t code[2][8];
+#pragma unroll 1
+        for (int round = 0; round < 2; ++round) {
+            bool near = false;
+            float worst = error;
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) worst = fmaxf(worst, __shfl_xor_sync(0xffffffffu, worst, o));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float lo = 0.f, hi = 0.f;
+                bool odd = false;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) lo = fminf(lo, x[8 * h + e]), hi = fmaxf(hi, x[8 * h + e]), odd = odd || !holds(x[8 * h + e]);
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) {
+                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                }
+                bad[h] = ((__ballot_sync(0xffffffffu, odd) >> (lane & 28)) & 15u) != 0;
+                scale[h] = scale_of(lo, hi, bad[h]);
+                const float margin = 0.5f - (worst * scale[h].inverse + 1.9073486e-06f);        // (2^-19: the quotients themselves)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float f = quotient(x[8 * h + e], scale[h].step, scale[h].inverse), k = rintf(f);
+                    code[h][e] = bad[h] ? 0u : (uint32_t)fminf(fmaxf(k + scale[h].zero, 0.f), 15.f);
+                    near = near || !(fabsf(f - k) <= margin);
+                }
+                // the step and the zero point
+                const float z = quotient(-lo, scale[h].step, scale[h].inverse);
+                const float range = hi - lo, slack = 2.f * worst + range * 4.7683716e-07f;       // (2^-21)
+                const uint32_t below = __float_as_uint(fmaxf((range - slack) * (1.f / 15.f), 0.f)) + 0xfffffu, above = __float_as_uint((range + slack) * (1.f / 15.f)) + 0xfffffu;
+                near = near || !(fabsf(z - rintf(z)) <= margin) || ((below ^ above) & ~0xfffffu) != 0 || !(fmaxf(hi, -lo) < 8.507059e37f);     // 2^126
+            }
+            if (round == 1 || !__any_sync(0xffffffffu, near && kind == 1 && worst != 0.f)) break;
+            // a key is near a border: all keys of the pass again, in 64 bits
+            double ss = 0.0, factor = 1.0;
+            if (has_norm) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const double a = stored ? (double)to_f32(first[p].v[e]) : 0.0, b = stored ? (double)to_f32(second[p].v[e]) : 0.0;
+                    ss += a * a + b * b;
+                }
+#pragma unroll
+                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                factor = 1.0 / sqrt(ss / (double)D + (double)eps);
+            }
+            if (kind == 1) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    double a = (double)to_f32(first[p].v[e]), b = (double)to_f32(second[p].v[e]);
+                    if (has_norm) a = a * factor * (double)s_gain[1][8 * li + e], b = b * factor * (double)s_gain[1][D / 2 + 8 * li + e];
+                    if (has_rope) {
+                        const double c = cs[2 * e], s = cs[2 * e + 1];
+                        x[e] = (float)(a * c - b * s);
+                        x[8 + e] = (float)(b * c + a * s);
+                    } else {
+                        x[e] = (float)a, x[8 + e] = (float)b;
+                    }
+                }
+                error = 0.f;
+            }
+        }
+        if (kind == 0 || !stored) continue;
+        unsigned char* block = block0 + (head - nq - (kind == 2 ? nkv : 0)) * head_bytes;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int g = (li >> 2) + h * (NG / 2), quarter = li & 3;
+            uint32_t word = 0;
+            if (kind == 1) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) word |= code[h][e] << (4 * (e >> 1) + 16 * (e & 1));
+                reinterpret_cast<uint32_t*>(block)[(token * 4 + quarter) * NG + g] = word;
+                if (quarter == 0) reinterpret_cast<uint16_t*>(block + key_words_at(D))[token * NG + g] = (uint16_t)scale[h].word;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) word |= code[h][e] << (4 * e);
+                uint16_t* codes = reinterpret_cast<uint16_t*>(block + value_codes_at(D)) +
+                                  ((((token >> 3) * 8 + 2 * quarter) * 4 + ((token & 7) >> 1)) * NG + g) * 2 + (token & 1);
+                codes[0] = (uint16_t)word;
+                codes[8 * NG] = (uint16_t)(word >> 16);
+                if (quarter == 0) reinterpret_cast<uint16_t*>(block + value_words_at(D))[((token >> 1) * NG + g) * 2 + (token & 1)] = (uint16_t)scale[h].word;
+            }
+        }
+    }
+}
+
+// The same head sizes with few tokens, or a rotation of a part of the head whose halves are whole lanes.  A lane has E = D / 32 neighbouring values of a
 // head, 32 / E lanes a group; a warp takes HB heads of one token: all their loads are issued at once, and what depends on the token only
 // (slot, position, table row, gains) is fetched once and before the wait for the kernel in front.  The rotation's partner
 // lies `rotary / 2 / E` lanes away; it is exchanged as it came, so that the exchange is exact, and normed again where it arrives.
-// Bound by the memory's latency at few tokens; at many by instructions: a key head costs about four times a query head (64-bit norm
-// and rotation, quantisation).
+// Bound by the memory's latency.
 template <typename T, int E, int HB>
 __global__ void __launch_bounds__(kWarps * 32)
 write_lanes_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, const int* __restrict__ positions, const int* __restrict__ slots, AnyVec q_gain,
@@ -329,6 +533,20 @@ static cudaError_t launch_write(int d, cudaStream_t stream, bool use_pdl, const 
                                 int num_pages, int page_size, int nq, int nkv, int num_tokens) {
     const int heads = nq + 2 * nkv;
     const bool many = (long long)num_tokens * heads >= kManyHeads;
+    if (many && (rotary == 0 || rotary == d) && (uintptr_t)qkv % 16 == 0 && (uintptr_t)q_out % 16 == 0 && (size_t)row_stride * sizeof(T) % 16 == 0 &&
+        (size_t)q_stride * sizeof(T) % 16 == 0) {
+        constexpr int P = sizeof(T) == 2 ? 2 : 1;
+        const int per_warp = 512 / d * P;                            // heads a warp takes
+        const long long row_warps = (long long)num_tokens * ((heads + per_warp - 1) / per_warp);
+        const dim3 rows((unsigned)((row_warps + kRowWarps - 1) / kRowWarps));
+#define CIB_KV4_ROWS(LV)                                                                                                                           \
+    return launch_pdl(write_rows_kernel<T, LV, P>, rows, dim3(kRowWarps * 32), 0, stream, use_pdl, qkv, row_stride, q_out, q_stride, positions, slots, qg, kg,  \
+                      has_norm, eps, rope_table, rotary > 0 ? 1 : 0, max_positions, cache, num_pages, page_size, nq, nkv, num_tokens)
+        if (d == 64) CIB_KV4_ROWS(4);
+        if (d == 128) CIB_KV4_ROWS(8);
+        CIB_KV4_ROWS(16);
+#undef CIB_KV4_ROWS
+    }
     const long long warps = (long long)num_tokens * ((heads + (many ? 3 : 0)) / (many ? 4 : 1));
     const dim3 grid((unsigned)((warps + kWarps - 1) / kWarps));
 #define CIB_KV4_WRITE(EV, HB)                                                                                                                      \

@@ -24,6 +24,21 @@ def quantise_group(x):
     return codes, (bits >> 16) | zero
 
 
+def held(x):
+    """What float32 values [..., d] are held as, float64: ``quantise_group`` for many groups at once."""
+    x = np.asarray(x, dtype=np.float32)
+    g = x.reshape(*x.shape[:-1], -1, 32)
+    good = (np.abs(g) < F(2.0 ** 127)).all(-1, keepdims=True)
+    g = np.where(good, g, F(0))
+    lo, hi = np.minimum(g.min(-1, keepdims=True), F(0)), np.maximum(g.max(-1, keepdims=True), F(0))
+    t = np.maximum((hi - lo) / F(15), F(2.0 ** -120))
+    step = ((t.view(np.uint32) + np.uint32(0xFFFFF)) & ~np.uint32(0xFFFFF)).view(np.float32)
+    zero = np.rint(-lo / step)
+    code = np.clip(np.rint(g / step) + zero, 0, 15)
+    out = step.astype(np.float64) * (code - zero).astype(np.float64)
+    return np.where(good, out, np.nan).reshape(x.shape)
+
+
 def value(code: int, word: int) -> float:
     """The number a code stands for (exact)."""
     step = float(np.array((word & 0xFFF0) << 16, dtype=np.uint32).view(np.float32)[()])

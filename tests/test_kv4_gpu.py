@@ -57,7 +57,10 @@ def rope_table(positions, rotary, theta=10000.0):
 WRITES = [  # T, nq, nkv, d, page, rotary, norm
     (1, 1, 1, 32, 16, 32, True), (3, 4, 2, 64, 16, 64, True), (17, 16, 8, 128, 16, 128, True), (40, 5, 1, 96, 48, 96, False),
     (300, 4, 2, 128, 32, 128, True), (257, 6, 3, 64, 16, 64, False), (9, 2, 2, 256, 16, 64, True), (300, 8, 4, 64, 64, 0, True),
-    (33, 3, 1, 160, 32, 20, True), (2049, 2, 1, 128, 16, 128, True), (513, 7, 3, 128, 16, 0, False)]
+    (33, 3, 1, 160, 32, 20, True), (2049, 2, 1, 128, 16, 128, True), (513, 7, 3, 128, 16, 0, False),
+    # enough heads for several to a warp
+    (1300, 4, 2, 128, 16, 128, True), (1201, 6, 3, 64, 16, 64, True), (1700, 2, 2, 256, 32, 256, True), (1300, 4, 2, 128, 16, 0, True),
+    (1300, 4, 2, 128, 16, 64, True), (1600, 5, 1, 128, 16, 128, False), (1600, 1, 3, 64, 48, 0, False)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -123,15 +126,20 @@ def test_write_and_read(dtype, sizes, order):
                     m[:, b] |= np.uint8(15 << s)
                 m[:, word], m[:, word + 1] = 255, 255
     assert not ((got.numpy() ^ want) & ~mask).any()
+    # ... every value of it
+    at = torch.tensor([s if s >= 0 else 0 for s in slots])
+    for rows, hold in zip((k, v), P4.unpack(cache, d)):
+        there = hold[at // page, :, at % page]
+        expect = torch.from_numpy(P4.held(rows.numpy().astype(np.float32)))
+        live = torch.tensor(slots) >= 0
+        assert torch.equal(there[live], expect[live])
     # reading back, in either type; a slot that is none leaves its row
     for kind in (F32, BF16):
         keys, values = (torch.full((T, nkv * d), -3.0, dtype=kind, device=DEV) for _ in range(2))
         kernels.kv4_read(cache, ints(slots), keys, values, nkv, d)
-        hold_k, hold_v = P4.unpack(cache, d)
-        for t, slot in enumerate(slots):
-            for got_row, hold in ((keys[t], hold_k), (values[t], hold_v)):
-                row = got_row.double().cpu().reshape(nkv, d)
-                assert torch.equal(row, hold[slot // page, :, slot % page]) if slot >= 0 else (row == -3).all()
+        for got_rows, hold in zip((keys, values), P4.unpack(cache, d)):
+            rows = got_rows.double().cpu().reshape(T, nkv, d)
+            assert torch.equal(rows[live], hold[at // page, :, at % page][live]) and (rows[~live] == -3).all()
     # in place: the queries of the rows are replaced, keys and values stay
     kernels.qk_norm_rope_kv4_write(dev, *args)
     assert torch.equal(dev[:, :nq * d], q_out) and torch.equal(dev[:, nq * d:].cpu(), qkv[:, nq * d:width]) and torch.equal(cache.cpu(), got)
