@@ -6,6 +6,8 @@
 //
 // The queries are computed in 32 bits, as where the cache is not quantised.  The keys' norm and rotation are computed in 64 bits: a value next
 // to the border between two codes would else fall to either side by the order of a sum, a difference of a whole step.
+#include <algorithm>
+
 #include "kv4.cuh"
 #include "mma_utils.cuh"
 
@@ -126,15 +128,112 @@ struct alignas(sizeof(T) * E > 16 ? 16 : sizeof(T) * E) Lane {
 // that bound of a border between two codes does it again in 64 bits: the codes are those of the 64-bit computation, which alone took
 // two thirds of the time.  The bound: the sum of squares is 8 + 8 additions deep at most (2^-21 of its root), the reciprocal root is good to 2
 // units (2^-22), two products, and the rotation's two products and sum: less than 2^-20.5 of |a cos| + |b sin| (2^-22.5 without a norm).
-constexpr int kRowWarps = 8;
+constexpr int kRowWarps = 8, kRowCtas = 2;          // CTAs an SM (three, which leave 80 registers, spill: 100 us for 8 001 tokens of 48 heads instead of 70)
 
 template <typename T>
 struct alignas(sizeof(T) * 8 > 16 ? 16 : sizeof(T) * 8) Eight {
     T v[8];
 };
 
+// Sixteen values of a lane (eight of either half; a group is four lanes of a half) as they are stored: the lane's codes and the groups' words.
+// `key`: in the order of key codes, else of value codes.  `worst`: how far values of the group may be off; returns whether a code, a zero point or
+// a step could be another one then.  Codes are small whole numbers: four of them are summed up by weight and converted at once.
+__device__ __forceinline__ bool quantise_lane(const float (&x)[16], bool key, float worst, int lane, uint32_t (&word)[2], uint32_t (&step)[2]) {
+    bool near = false;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float lo = 0.f, hi = 0.f, odd = 0.f;                         // odd: 0, or not a number where a value is not finite
+#pragma unroll
+        for (int e = 0; e < 8; ++e) lo = fminf(lo, x[8 * h + e]), hi = fmaxf(hi, x[8 * h + e]), odd = fmaf(x[8 * h + e], 0.f, odd);
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        const bool bad = ((__ballot_sync(0xffffffffu, !(odd == 0.f) || !holds(hi) || !holds(lo)) >> (lane & 28)) & 15u) != 0;
+        const Scale s = scale_of(lo, hi, bad);
+        float c[8], off = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float f = quotient(x[8 * h + e], s.step, s.inverse), k = rintf(f);
+            off = fmaxf(off, fabsf(f - k));
+            c[e] = fminf(fmaxf(k + s.zero, 0.f), 15.f);
+        }
+        float low, high;                                             // the halves of the lane's word
+        if (key) {
+            low = fmaf(fmaf(fmaf(c[6], 16.f, c[4]), 16.f, c[2]), 16.f, c[0]);
+            high = fmaf(fmaf(fmaf(c[7], 16.f, c[5]), 16.f, c[3]), 16.f, c[1]);
+        } else {
+            low = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]);
+            high = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]);
+        }
+        // (whole numbers below 2^16: adding 2^23 leaves them in the lowest bits)
+        word[h] = bad ? 0u : __byte_perm(__float_as_uint(low + 8388608.f), __float_as_uint(high + 8388608.f), 0x5410);
+        step[h] = s.word;
+        const float margin = 0.5f - (worst * s.inverse + 1.9073486e-06f);          // (2^-19: the quotients themselves)
+        const float z = quotient(-lo, s.step, s.inverse), range = hi - lo, slack = 2.f * worst + range * 4.7683716e-07f;       // (2^-21)
+        const uint32_t below = __float_as_uint(fmaxf((range - slack) * (1.f / 15.f), 0.f)) + 0xfffffu, above = __float_as_uint((range + slack) * (1.f / 15.f)) + 0xfffffu;
+        near = near || !(fmaxf(off, fabsf(z - rintf(z))) <= margin) || ((below ^ above) & ~0xfffffu) != 0 || !(fmaxf(hi, -lo) < 8.507059e37f) || !(odd == 0.f);     // 2^126
+    }
+    return near;
+}
+// ... and where they go: `li` is the lane within its head.
+template <int D>
+__device__ __forceinline__ void store_lane(unsigned char* block, bool key, int token, int li, const uint32_t (&word)[2], const uint32_t (&step)[2]) {
+    constexpr int NG = D / kGroup;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int g = (li >> 2) + h * (NG / 2), quarter = li & 3;
+        if (key) {
+            reinterpret_cast<uint32_t*>(block)[(token * 4 + quarter) * NG + g] = word[h];
+            if (quarter == 0) reinterpret_cast<uint16_t*>(block + key_words_at(D))[token * NG + g] = (uint16_t)step[h];
+        } else {
+            uint16_t* codes = reinterpret_cast<uint16_t*>(block + value_codes_at(D)) +
+                              ((((token >> 3) * 8 + 2 * quarter) * 4 + ((token & 7) >> 1)) * NG + g) * 2 + (token & 1);
+            codes[0] = (uint16_t)word[h];
+            codes[8 * NG] = (uint16_t)(word[h] >> 16);
+            if (quarter == 0) reinterpret_cast<uint16_t*>(block + value_words_at(D))[((token >> 1) * NG + g) * 2 + (token & 1)] = (uint16_t)step[h];
+        }
+    }
+}
+// The key heads of a pass in 64 bits (a call of its own: few warps need it, and its registers would cost all of them).
+template <typename T, int L>
+__device__ __noinline__ void write_keys_exactly(const T* src, bool mine, const float* gain, int has_norm, float eps, const float* table, int has_rope,
+                                                unsigned char* block, int token, int li) {
+    constexpr int D = 16 * L;
+    const Eight<T> first = *reinterpret_cast<const Eight<T>*>(src), second = *reinterpret_cast<const Eight<T>*>(src + D / 2);
+    double factor = 1.0;
+    if (has_norm) {
+        double ss = 0.0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const double a = to_f32(first.v[e]), b = to_f32(second.v[e]);
+            ss += a * a + b * b;
+        }
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        factor = 1.0 / sqrt(ss / (double)D + (double)eps);
+    }
+    float x[16];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        double a = to_f32(first.v[e]), b = to_f32(second.v[e]);
+        if (has_norm) a = a * factor * (double)gain[8 * li + e], b = b * factor * (double)gain[D / 2 + 8 * li + e];
+        if (has_rope) {
+            const double c = table[16 * li + 2 * e], s = table[16 * li + 2 * e + 1];
+            x[e] = (float)(a * c - b * s);
+            x[8 + e] = (float)(b * c + a * s);
+        } else {
+            x[e] = (float)a, x[8 + e] = (float)b;
+        }
+    }
+    uint32_t word[2], step[2];
+    quantise_lane(x, true, 0.f, threadIdx.x & 31, word, step);
+    if (mine) store_lane<D>(block, true, token, li, word, step);
+}
+
 template <typename T, int L, int PASSES>
-__global__ void __launch_bounds__(kRowWarps * 32)
+__global__ void __launch_bounds__(kRowWarps * 32, kRowCtas)
 write_rows_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, const int* __restrict__ positions, const int* __restrict__ slots, AnyVec q_gain,
                   AnyVec k_gain, int has_norm, float eps, const float* __restrict__ rope_table, int has_rope, int max_positions,
                   unsigned char* __restrict__ cache, int num_pages, int page_size, int nq, int nkv, int num_tokens) {
@@ -144,28 +243,29 @@ write_rows_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, const in
         for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) s_gain[i / D][i % D] = i < D ? q_gain[i] : k_gain[i - D];
     const int lane = threadIdx.x & 31, sub = lane / L, li = lane % L;
     const int heads = nq + 2 * nkv, chunks = (heads + HPP * PASSES - 1) / (HPP * PASSES);
-    const int w = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-    const int t = w / chunks, base = (w - t * chunks) * HPP * PASSES;
-    const bool live = t < num_tokens;
-    float cs[16];
-    int slot = -1;
-    if (live) {
-        slot = slots[t];
-        if (has_rope) {
-            int pos = positions[t];
-            pos = pos < 0 ? 0 : (pos >= max_positions ? max_positions - 1 : pos);
-            const float4* tp = reinterpret_cast<const float4*>(rope_table + (size_t)pos * D + 16 * li);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float4 v = tp[e];
-                cs[4 * e] = v.x, cs[4 * e + 1] = v.y, cs[4 * e + 2] = v.z, cs[4 * e + 3] = v.w;
-            }
-        }
-    }
+    const size_t head_bytes = (size_t)(page_size / kBlock) * block_bytes(D);
     griddep_wait();
     griddep_launch();
     __syncthreads();
-    if (!live) return;
+    // the launch has as many CTAs as the GPU holds: a warp goes on with the next piece of work instead of leaving and another starting
+    const long long pieces = (long long)num_tokens * chunks;
+    for (long long w = (long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5); w < pieces; w += (long long)gridDim.x * kRowWarps) {
+    const int t = (int)(w / chunks), base = (int)(w - (long long)t * chunks) * HPP * PASSES;
+    float cs[16];
+    unsigned again = 0;                                              // passes with a key near a border
+    const float* rope_row = rope_table;
+    const int slot = slots[t];
+    if (has_rope) {
+        int pos = positions[t];
+        pos = pos < 0 ? 0 : (pos >= max_positions ? max_positions - 1 : pos);
+        rope_row = rope_table + (size_t)pos * D;
+        const float4* tp = reinterpret_cast<const float4*>(rope_row + 16 * li);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float4 v = tp[e];
+            cs[4 * e] = v.x, cs[4 * e + 1] = v.y, cs[4 * e + 2] = v.z, cs[4 * e + 3] = v.w;
+        }
+    }
     const T* src = qkv + (size_t)t * row_stride + 8 * li;
     Eight<T> first[PASSES], second[PASSES];
 #pragma unroll
@@ -177,7 +277,6 @@ write_rows_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, const in
         }
     }
     unsigned char* block0 = block_of(cache, slot, num_pages, page_size, nkv, 0, D);
-    const size_t head_bytes = (size_t)(page_size / kBlock) * block_bytes(D);
     const int token = block0 == nullptr ? 0 : slot % page_size % kBlock;
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
@@ -234,92 +333,22 @@ write_rows_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, const in
             *reinterpret_cast<Eight<T>*>(dst + D / 2) = b;
         }
         if (block0 == nullptr || !__any_sync(0xffffffffu, kind != 0)) continue;
-        // ---- quantisation: groups are four lanes of either half ----
-        Scale scale[2];
-        bool bad[2];
-        uint32_t code[2][8];
-#pragma unroll 1
-        for (int round = 0; round < 2; ++round) {
-            bool near = false;
-            float worst = error;
+        uint32_t word[2], step[2];
 #pragma unroll
-            for (int o = 1; o < 4; o <<= 1) worst = fmaxf(worst, __shfl_xor_sync(0xffffffffu, worst, o));
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float lo = 0.f, hi = 0.f;
-                bool odd = false;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) lo = fminf(lo, x[8 * h + e]), hi = fmaxf(hi, x[8 * h + e]), odd = odd || !holds(x[8 * h + e]);
-#pragma unroll
-                for (int o = 1; o < 4; o <<= 1) {
-                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-                }
-                bad[h] = ((__ballot_sync(0xffffffffu, odd) >> (lane & 28)) & 15u) != 0;
-                scale[h] = scale_of(lo, hi, bad[h]);
-                const float margin = 0.5f - (worst * scale[h].inverse + 1.9073486e-06f);        // (2^-19: the quotients themselves)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float f = quotient(x[8 * h + e], scale[h].step, scale[h].inverse), k = rintf(f);
-                    code[h][e] = bad[h] ? 0u : (uint32_t)fminf(fmaxf(k + scale[h].zero, 0.f), 15.f);
-                    near = near || !(fabsf(f - k) <= margin);
-                }
-                // the step and the zero point
-                const float z = quotient(-lo, scale[h].step, scale[h].inverse);
-                const float range = hi - lo, slack = 2.f * worst + range * 4.7683716e-07f;       // (2^-21)
-                const uint32_t below = __float_as_uint(fmaxf((range - slack) * (1.f / 15.f), 0.f)) + 0xfffffu, above = __float_as_uint((range + slack) * (1.f / 15.f)) + 0xfffffu;
-                near = near || !(fabsf(z - rintf(z)) <= margin) || ((below ^ above) & ~0xfffffu) != 0 || !(fmaxf(hi, -lo) < 8.507059e37f);     // 2^126
-            }
-            if (round == 1 || !__any_sync(0xffffffffu, near && kind == 1 && worst != 0.f)) break;
-            // a key is near a border: all keys of the pass again, in 64 bits
-            double ss = 0.0, factor = 1.0;
-            if (has_norm) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const double a = stored ? (double)to_f32(first[p].v[e]) : 0.0, b = stored ? (double)to_f32(second[p].v[e]) : 0.0;
-                    ss += a * a + b * b;
-                }
-#pragma unroll
-                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                factor = 1.0 / sqrt(ss / (double)D + (double)eps);
-            }
-            if (kind == 1) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    double a = (double)to_f32(first[p].v[e]), b = (double)to_f32(second[p].v[e]);
-                    if (has_norm) a = a * factor * (double)s_gain[1][8 * li + e], b = b * factor * (double)s_gain[1][D / 2 + 8 * li + e];
-                    if (has_rope) {
-                        const double c = cs[2 * e], s = cs[2 * e + 1];
-                        x[e] = (float)(a * c - b * s);
-                        x[8 + e] = (float)(b * c + a * s);
-                    } else {
-                        x[e] = (float)a, x[8 + e] = (float)b;
-                    }
-                }
-                error = 0.f;
-            }
-        }
-        if (kind == 0 || !stored) continue;
-        unsigned char* block = block0 + (head - nq - (kind == 2 ? nkv : 0)) * head_bytes;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int g = (li >> 2) + h * (NG / 2), quarter = li & 3;
-            uint32_t word = 0;
-            if (kind == 1) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) word |= code[h][e] << (4 * (e >> 1) + 16 * (e & 1));
-                reinterpret_cast<uint32_t*>(block)[(token * 4 + quarter) * NG + g] = word;
-                if (quarter == 0) reinterpret_cast<uint16_t*>(block + key_words_at(D))[token * NG + g] = (uint16_t)scale[h].word;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) word |= code[h][e] << (4 * e);
-                uint16_t* codes = reinterpret_cast<uint16_t*>(block + value_codes_at(D)) +
-                                  ((((token >> 3) * 8 + 2 * quarter) * 4 + ((token & 7) >> 1)) * NG + g) * 2 + (token & 1);
-                codes[0] = (uint16_t)word;
-                codes[8 * NG] = (uint16_t)(word >> 16);
-                if (quarter == 0) reinterpret_cast<uint16_t*>(block + value_words_at(D))[((token >> 1) * NG + g) * 2 + (token & 1)] = (uint16_t)scale[h].word;
-            }
-        }
+        for (int o = 1; o < 4; o <<= 1) error = fmaxf(error, __shfl_xor_sync(0xffffffffu, error, o));
+        const bool near = quantise_lane(x, kind == 1, error, lane, word, step);
+        if (__any_sync(0xffffffffu, near && kind == 1 && error != 0.f)) again |= 1u << p;
+        if (kind != 0 && stored) store_lane<D>(block0 + (head - nq - (kind == 2 ? nkv : 0)) * head_bytes, kind == 1, token, li, word, step);
+    }
+    // keys near a border: the pass's key heads again (a lane stores to where it stored before)
+    while (again != 0) {
+        const int p = __ffs(again) - 1;
+        again &= again - 1;
+        const int head = base + p * HPP + sub;
+        const bool mine = head >= nq && head < nq + nkv;
+        write_keys_exactly<T, L>(src + (size_t)(mine ? head : nq) * D, mine, s_gain[1], has_norm, eps, rope_row, has_rope,
+                                 block0 + (mine ? head - nq : 0) * head_bytes, token, li);
+    }
     }
 }
 
@@ -538,7 +567,7 @@ static cudaError_t launch_write(int d, cudaStream_t stream, bool use_pdl, const 
         constexpr int P = sizeof(T) == 2 ? 2 : 1;
         const int per_warp = 512 / d * P;                            // heads a warp takes
         const long long row_warps = (long long)num_tokens * ((heads + per_warp - 1) / per_warp);
-        const dim3 rows((unsigned)((row_warps + kRowWarps - 1) / kRowWarps));
+        const dim3 rows((unsigned)std::min<long long>((row_warps + kRowWarps - 1) / kRowWarps, 148 * kRowCtas));
 #define CIB_KV4_ROWS(LV)                                                                                                                           \
     return launch_pdl(write_rows_kernel<T, LV, P>, rows, dim3(kRowWarps * 32), 0, stream, use_pdl, qkv, row_stride, q_out, q_stride, positions, slots, qg, kg,  \
                       has_norm, eps, rope_table, rotary > 0 ? 1 : 0, max_positions, cache, num_pages, page_size, nq, nkv, num_tokens)
