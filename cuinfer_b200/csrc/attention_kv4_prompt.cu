@@ -2,8 +2,9 @@
 //
 //   * A CTA has an SM alone and owns two tiles of 128 rows (query token x query head of one kv head) that walk the same 64-key tiles:
 //     what taking a key tile apart costs is shared by 256 rows.
-//   * Eight warps take the codes apart, four the keys and four the values (four for both were the bottleneck: 2 450 cycles a key tile). Blocks
-//     come by bulk copies (`cp.async.bulk`, three key tiles ahead); a warp's lanes read 16 bytes of codes each and write bfloat16 numbers into
+//   * Eight warps take the codes apart, four the keys and four the values (four for both were the bottleneck: 2 450 cycles a key tile).  A warp's
+//     lanes read 16 bytes of codes each straight from global memory, a tile ahead (through bulk copies into shared memory the copies' barriers took
+//     as long as the arithmetic), and write bfloat16 numbers into
 //     the tiles that the tensor cores read (128-byte swizzle).  step * (code - zero) is exact in bfloat16, so these are the cache's
 //     numbers.  Keys are a K-major operand, [key][value column]; values too, but transposed, [value column][key]: a word of value codes
 //     holds two neighbouring keys of a column, which is the order that operand has.
@@ -31,10 +32,12 @@ using namespace kv4;
 constexpr int kM = 128;               // rows of a tile
 constexpr int kN = 64;                // keys of a tile
 constexpr int kSoftWarps = 8;         // four to a row tile
-constexpr int kMmaWarp = kSoftWarps;
 constexpr int kTakeWarps = 4;         // take the keys apart, and as many the values
-constexpr int kThreads = (kSoftWarps + 1 + 2 * kTakeWarps) * 32;
-constexpr int kRawStages = 4;         // key tiles as bytes: three on their way, one being read
+constexpr int kMmaWarp = kSoftWarps + 2 * kTakeWarps;          // two of them: one for each row tile
+constexpr int kThreads = (kMmaWarp + 2) * 32;
+// Registers a thread: the launch gives every warp 96 (18 warps take the place of 20); the softmax warps get 24 of each taking warp's.
+constexpr int kLaunchRegs = 96, kSoftRegs = 120, kTakeRegs = 72;
+static_assert(kSoftWarps * kSoftRegs + 2 * kTakeWarps * kTakeRegs == (kSoftWarps + 2 * kTakeWarps) * kLaunchRegs, "no warp may wait for registers that are not there");
 constexpr int kTmemCols = 512;        // per row tile: S of even key tiles | S of odd ones | O
 
 constexpr uint32_t kMinus2p127 = 0xff00ff00u, k2p127 = 0x7f007f00u, k2p123 = 0x7d007d00u, k64 = 0x42804280u;
@@ -76,10 +79,6 @@ __device__ __forceinline__ void tst32(uint32_t taddr, const uint32_t (&r)[32]) {
           "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(tc_smem_u32(dst)), "l"(src), "r"(bytes), "r"(tc_smem_u32(bar)) : "memory");
-}
 // two 32-bit numbers at a time
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;
@@ -112,9 +111,7 @@ template <int D>
 struct Smem {
     static constexpr int kPanels = D / 64;                         // 64-column panels of a query or key row
     static constexpr int kQ = kPanels * kM * 128, kK = kPanels * kN * 128, kV = D * 128;
-    static constexpr int kRawBlock = block_bytes(D) + 32;          // (padded: the four blocks of a tile start in different banks)
-    static constexpr int kRaw = 2 * kQ + 2 * kK + 2 * kV;
-    static constexpr int kBars = kRaw + kRawStages * (kN / kBlock) * kRawBlock;
+    static constexpr int kBars = 2 * kQ + 2 * kK + 2 * kV;
     static constexpr int kTotal = kBars + 256 + 1024;
 };
 
@@ -138,13 +135,11 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
     uint64_t* s_full = bars + 4;        // [row tile][2] S of a key tile is in tensor memory: its keys' buffer is free
     uint64_t* p_ready = bars + 8;       // [row tile][2] P is (the softmax warps arrive)
     uint64_t* pv_done = bars + 12;      // [row tile][2] O includes a key tile: its values' buffer is free
-    uint64_t* raw_full = bars + 16;     // [stages] a key tile's blocks have landed
-    uint64_t* raw_free = raw_full + kRawStages;     // [stages] the taking warps have read them
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_free + kRawStages);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
     __shared__ int s_req, s_pair, s_abort, s_q0, s_n, s_seq;
-    // Which of a key tile's blocks the table does not name, tile j at j % 8: written three tiles ahead, when P V of tile j - 5 at least is done, and
-    // read up to P V of tile j.
-    __shared__ int s_missing[8];
+    // Which of a key tile's blocks the table does not name, tile j at j % 4: written when S of tile j - 2 is there, so P V of tile j - 4 was issued and
+    // every row is through with that tile.
+    __shared__ int s_missing[4];
     __shared__ int s_odd;               // a value that is not a number has been met
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -186,12 +181,12 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
                 s_seq = seq_lens[req];
             }
         }
-    } else if (warp == 1 && lane < 16 + 2 * kRawStages) {
-        mbar_init(&bars[lane], lane >= 16 + kRawStages ? 2 * kTakeWarps : lane < 4 || lane >= 16 ? kTakeWarps : lane >= 8 && lane < 12 ? 4 : 1);
+    } else if (warp == 1 && lane < 16) {
+        mbar_init(&bars[lane], lane < 4 ? kTakeWarps : lane >= 8 && lane < 12 ? 4 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (tid < 8) s_missing[tid] = 0;
+    if (tid < 4) s_missing[tid] = 0;
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem_u32(tmem_slot)), "r"((uint32_t)kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -246,7 +241,7 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp <= kMmaWarp) asm volatile("bar.sync 10, %0;" ::"r"((kMmaWarp + 1) * 32) : "memory");
+    if (warp < kSoftWarps || warp >= kMmaWarp) asm volatile("bar.sync 10, %0;" ::"r"((kSoftWarps + 2) * 32) : "memory");
 
     auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
         bool ok = mbar_try_wait(bar, parity) || (*(volatile int*)&s_abort == 0 && mbar_wait(bar, parity));
@@ -254,166 +249,183 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
         return __all_sync(0xffffffffu, ok) != 0;
     };
 
-    if (active && warp == kMmaWarp) {
-        // ---- the MMAs: the whole warp walks the loop, one lane issues.  Addresses are broadcast, so that the compiler knows them to be the
-        // warp's and keeps them in uniform registers (out of per-thread ones an MMA took 72 cycles to issue) ----
-        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-        const uint32_t aq = __shfl_sync(0xffffffffu, tc_smem_u32(sQ), 0), ak = __shfl_sync(0xffffffffu, tc_smem_u32(sK), 0), av = __shfl_sync(0xffffffffu, tc_smem_u32(sV), 0);
+    if (active && warp >= kMmaWarp) {
+        // ---- the MMAs: a warp for each row tile walks its loop, one lane issues (one warp for both was busy for 2 350 of 2 450 cycles a key
+        // tile).  Addresses are broadcast, so that the compiler knows them to be the warp's and keeps them in uniform registers (out of
+        // per-thread ones an MMA took 72 cycles to issue) ----
+        const int t = __shfl_sync(0xffffffffu, warp - kMmaWarp, 0);
+        const int my_tiles = t == 0 ? tiles[0] : tiles[1];
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + t * 256;
+        const uint32_t aq = __shfl_sync(0xffffffffu, tc_smem_u32(sQ), 0) + t * S::kQ, ak = __shfl_sync(0xffffffffu, tc_smem_u32(sK), 0), av = __shfl_sync(0xffffffffu, tc_smem_u32(sV), 0);
         const bool elected = elect_one();
-        auto issue_s = [&](int t, int j) {
+        auto issue_s = [&](int j) {
             const int b = j & 1;
             if (elected) {
-                const uint64_t qd = desc_k_major(aq + t * S::kQ), kd = desc_k_major(ak + b * S::kK);
+                const uint64_t qd = desc_k_major(aq), kd = desc_k_major(ak + b * S::kK);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     const uint64_t q_off = (uint64_t)(((k >> 2) * (kM * 128) + (k & 3) * 32) >> 4), k_off = (uint64_t)(((k >> 2) * (kN * 128) + (k & 3) * 32) >> 4);
-                    umma_bf16(tm + (uint32_t)(t * 256 + b * kN), qd + q_off, kd + k_off, idesc(kN), k != 0);
+                    umma_bf16(tm + (uint32_t)(b * kN), qd + q_off, kd + k_off, idesc(kN), k != 0);
                 }
                 umma_commit(&s_full[t * 2 + b]);
             }
             __syncwarp();
         };
         bool ok = true;
-        if (most > 0) {
+        if (my_tiles > 0) {
             ok = wait_all(&k_full[0], 0, 51);
             if (ok) {
                 tcgen05_fence_after();
-                if (tiles[0] > 0) issue_s(0, 0);
-                if (tiles[1] > 0) issue_s(1, 0);
+                issue_s(0);
             }
         }
-        for (int j = 0; j < most && ok; ++j) {
+        for (int j = 0; j < my_tiles && ok; ++j) {
             const int b = j & 1;
             const uint32_t parity = (j >> 1) & 1;
-            if (j + 1 < most) {
+            if (j + 1 < my_tiles) {
                 // S(j + 1) overwrites S and P of tile j - 1: P V(j - 1) was issued before, and the tensor pipe runs what one thread issues in order
                 ok = wait_all(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, 52);
                 if (!ok) break;
                 tcgen05_fence_after();
-                if (j + 1 < tiles[0]) issue_s(0, j + 1);
-                if (j + 1 < tiles[1]) issue_s(1, j + 1);
+                issue_s(j + 1);
             }
-            ok = wait_all(&v_full[b], parity, 53);
+            ok = wait_all(&v_full[b], parity, 53) && wait_all(&p_ready[t * 2 + b], parity, 54);
             if (!ok) break;
+            tcgen05_fence_after();
+            if (elected) {
+                const uint64_t vd = desc_k_major(av + b * S::kV);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                if (j >= tiles[t] || !ok) continue;
-                ok = wait_all(&p_ready[t * 2 + b], parity, 54);
-                if (!ok) continue;
-                tcgen05_fence_after();
-                if (elected) {
-                    const uint64_t vd = desc_k_major(av + b * S::kV);
-#pragma unroll
-                    for (int k = 0; k < kN / 16; ++k)
-                        mma_ts(tm + (uint32_t)(t * 256 + 2 * kN), tm + (uint32_t)(t * 256 + b * kN + k * 8), vd + (uint64_t)(k * 32 >> 4), idesc(D), j > 0 || k != 0);
-                    umma_commit(&pv_done[t * 2 + b]);
-                }
-                __syncwarp();
+                for (int k = 0; k < kN / 16; ++k)
+                    mma_ts(tm + (uint32_t)(2 * kN), tm + (uint32_t)(b * kN + k * 8), vd + (uint64_t)(k * 32 >> 4), idesc(D), j > 0 || k != 0);
+                umma_commit(&pv_done[t * 2 + b]);
             }
+            __syncwarp();
         }
-    } else if (active && warp > kMmaWarp) {
-        // ---- taking the codes apart: warps 0-3 of these the keys (and asking for the blocks), 4-7 the values ----
-        const int take = (warp - kMmaWarp - 1) & 3;
-        const bool values = warp - kMmaWarp - 1 >= kTakeWarps;
-        unsigned char* raw = base + S::kRaw;
-        // a tile's buffer b is free when the last row tile that had tile j - 2 is through with it (one thread issues the MMAs in order)
+    } else if (active && warp >= kSoftWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTakeRegs));
+        // ---- taking the codes apart: warps 0-3 of these the keys, 4-7 the values ----
+        const int take = (warp - kSoftWarps) & 3;
+        const bool values = warp >= kSoftWarps + kTakeWarps;
+        const int* table = block_table + (size_t)r * table_stride;
+        const int per_page = page_size / kBlock;
+        // the number of block `block` of key tile j, or -1 (no such tile, behind the last key, or not named by the table)
+        auto lookup = [&](int j, int block) {
+            const int b = (k_lo + j * kN) / kBlock + block, index = b / per_page;
+            if (j >= most || b * kBlock >= seq_len || index >= table_stride) return -1;
+            const int page = __ldg(table + index);
+            return page >= 0 && page < num_pages ? (page * nkv + kvh) * per_page + (b - index * per_page) : -1;
+        };
+        // a tile's buffer is free when both row tiles are through with tile j - 2
         auto free_again = [&](uint64_t* bars2, int j, int code) {
-            return j < 2 || wait_all(&bars2[(j - 2 < tiles[1] ? 2 : 0) + (j & 1)], (uint32_t)(((j >> 1) - 1) & 1), code);
+            const uint32_t parity = (uint32_t)(((j >> 1) - 1) & 1);
+            return (j - 2 < 0 || j - 2 >= tiles[0] || wait_all(&bars2[j & 1], parity, code)) && (j - 2 < 0 || j - 2 >= tiles[1] || wait_all(&bars2[2 + (j & 1)], parity, code + 1));
         };
         if (!values) {
-            const int* table = block_table + (size_t)r * table_stride;
-            const int per_page = page_size / kBlock;
             // a warp has one of the tile's four blocks; lane = (token, quarter), tokens in the order 0 4 1 5 2 6 3 7 so that the 16-byte stores
             // of eight lanes meet in no bank
             const int quarter = lane & 3, token = ((lane >> 3) & 3) + ((lane >> 2) & 1) * 4;
-            auto lookup = [&](int j) {
-                const int b = (k_lo + j * kN) / kBlock + take, index = b / per_page;
-                if (j >= most || b * kBlock >= seq_len || index >= table_stride) return -1;
-                const int page = __ldg(table + index);
-                return page >= 0 && page < num_pages ? (page * nkv + kvh) * per_page + (b - index * per_page) : -1;
+            struct Codes {
+                Words<NG> c[2];
+                Words<HG> w[2];
+                int id;
             };
-            // what the table does not name is not copied
-            int ids = -1;                                           // lane l: this warp's block of tile 32 n + l
-            auto request = [&](int j) {
-                if ((j & 31) == 0) ids = lookup(j + lane);
-                if (j >= most || lane != (j & 31)) return;
-                const int stage = j % kRawStages;
-                if (ids < 0 && k_lo + j * kN + take * kBlock < seq_len) atomicOr(&s_missing[j & 7], 1 << take);
-                else atomicAnd(&s_missing[j & 7], ~(1 << take));
-                mbar_expect_tx(&raw_full[stage], ids >= 0 ? kBytes : 0);
-                if (ids >= 0) bulk_load(raw + (stage * (kN / kBlock) + take) * S::kRawBlock, cache + (size_t)ids * kBytes, kBytes, &raw_full[stage]);
-            };
+            int ids = lookup(lane, take), ids_next = -1;            // lane l: this warp's block of tile 32 n + l
+            auto load = [&](int j) {
+                Codes x;
+                if ((j & 31) == 0 && j != 0) ids = ids_next;
+                if ((j & 31) == 16) ids_next = lookup((j & ~31) + 32 + lane, take);
+                x.id = __shfl_sync(0xffffffffu, ids, j & 31);
+                const unsigned char* kb = cache + (size_t)max(x.id, 0) * kBytes;       // (a block that is not there: any other, its scores are replaced)
 #pragma unroll
-            for (int i = 0; i < kRawStages - 1; ++i) request(i);
+                for (int h = 0; h < 2; ++h) {
+                    x.c[h] = reinterpret_cast<const Words<NG>*>(kb)[(token + 8 * h) * 4 + quarter];
+                    x.w[h] = reinterpret_cast<const Words<HG>*>(kb + key_words_at(D))[token + 8 * h];
+                }
+                return x;
+            };
+            Codes next = load(0);
             for (int j = 0; j < most; ++j) {
                 const int b = j & 1;
-                // the stage of tile j - 1 is refilled once all warps have read it
-                if (j > 0 && !wait_all(&raw_free[(j - 1) % kRawStages], (uint32_t)(((j - 1) / kRawStages) & 1), 64)) break;
-                request(j + kRawStages - 1);
-                __syncwarp();
-                if (!wait_all(&raw_full[j % kRawStages], (uint32_t)((j / kRawStages) & 1), 63)) break;
-                const unsigned char* kb = raw + ((j % kRawStages) * (kN / kBlock) + take) * S::kRawBlock;
+                const Codes x = next;
+                if (j + 1 < most) next = load(j + 1);
                 if (!free_again(s_full, j, 55)) break;
+                if (lane == 0) {
+                    if (x.id < 0 && k_lo + j * kN + take * kBlock < seq_len) atomicOr(&s_missing[j & 3], 1 << take);
+                    else atomicAnd(&s_missing[j & 3], ~(1 << take));
+                }
                 unsigned char* kt = sK + b * S::kK;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int row = take * kBlock + token + 8 * h;
-                    const Words<NG> kc = reinterpret_cast<const Words<NG>*>(kb)[(token + 8 * h) * 4 + quarter];
-                    const Words<HG> kw = reinterpret_cast<const Words<HG>*>(kb + key_words_at(D))[token + 8 * h];
 #pragma unroll
                     for (int k = 0; k < NG; ++k) {
-                        const uint32_t w = k & 1 ? __byte_perm(kw.w[k >> 1], 0, 0x3232) : __byte_perm(kw.w[k >> 1], 0, 0x1010);
+                        const uint32_t w = k & 1 ? __byte_perm(x.w[h].w[k >> 1], 0, 0x3232) : __byte_perm(x.w[h].w[k >> 1], 0, 0x1010);
                         const uint32_t zero = mul_bf16x2(w & 0x000f000fu, kMinus2p127), step = mul_bf16x2(w & 0xfff0fff0u, k64);
-                        const uint32_t x = kc.w[k], y = x >> 8;
+                        const uint32_t lo = x.c[h].w[k], hi = lo >> 8;
                         uint4 v;
-                        v.x = mul_bf16x2(fma_bf16x2(x & 0x000f000fu, k2p127, zero), step);
-                        v.y = mul_bf16x2(fma_bf16x2(x & 0x00f000f0u, k2p123, zero), step);
-                        v.z = mul_bf16x2(fma_bf16x2(y & 0x000f000fu, k2p127, zero), step);
-                        v.w = mul_bf16x2(fma_bf16x2(y & 0x00f000f0u, k2p123, zero), step);
+                        v.x = mul_bf16x2(fma_bf16x2(lo & 0x000f000fu, k2p127, zero), step);
+                        v.y = mul_bf16x2(fma_bf16x2(lo & 0x00f000f0u, k2p123, zero), step);
+                        v.z = mul_bf16x2(fma_bf16x2(hi & 0x000f000fu, k2p127, zero), step);
+                        v.w = mul_bf16x2(fma_bf16x2(hi & 0x00f000f0u, k2p123, zero), step);
                         *reinterpret_cast<uint4*>(kt + (k >> 1) * (kN * 128) + row * 128 + ((((k & 1) * 4 + quarter) ^ (row & 7)) << 4)) = v;
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&k_full[b]), mbar_arrive(&raw_free[j % kRawStages]);
+                if (lane == 0) mbar_arrive(&k_full[b]);
             }
         } else {
             // lane = (eight keys, eighth of a group); a warp has half of the eighths and half of the groups
             const int octet = lane & 7, eighth = (take >> 1) * 4 + (lane >> 3), g0 = (take & 1) * HG;
+            struct Codes {
+                Words<HG> c[4], w[4];
+            };
+            // lanes 4 i .. 4 i + 3: the blocks of tile 8 n + i
+            int ids = lookup(lane >> 2, lane & 3), ids_next = -1;
+            auto load = [&](int j) {
+                Codes x;
+                if ((j & 7) == 0 && j != 0) ids = ids_next;
+                if ((j & 7) == 4) ids_next = lookup((j & ~7) + 8 + (lane >> 2), lane & 3);
+                const int id = __shfl_sync(0xffffffffu, ids, (j & 7) * 4 + (octet >> 1));
+                const unsigned char* vb = cache + (size_t)max(id, 0) * kBytes;
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    x.c[p] = reinterpret_cast<const Words<HG>*>(vb + value_codes_at(D))[(((octet & 1) * 8 + eighth) * 4 + p) * 2 + (take & 1)];
+                    x.w[p] = reinterpret_cast<const Words<HG>*>(vb + value_words_at(D))[((octet & 1) * 4 + p) * 2 + (take & 1)];
+                    if (id < 0)                                     // of no page: the weights are zero
+#pragma unroll
+                        for (int k = 0; k < HG; ++k) x.w[p].w[k] = 0;
+                }
+                return x;
+            };
+            Codes next = load(0);
             for (int j = 0; j < most; ++j) {
                 const int b = j & 1;
                 const int key0 = k_lo + j * kN;
-                if (!wait_all(&raw_full[j % kRawStages], (uint32_t)((j / kRawStages) & 1), 65)) break;
-                const unsigned char* vb = raw + ((j % kRawStages) * (kN / kBlock) + (octet >> 1)) * S::kRawBlock;
-                Words<HG> vc[4], vw[4];
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    vc[p] = reinterpret_cast<const Words<HG>*>(vb + value_codes_at(D))[(((octet & 1) * 8 + eighth) * 4 + p) * 2 + (take & 1)];
-                    vw[p] = reinterpret_cast<const Words<HG>*>(vb + value_words_at(D))[((octet & 1) * 4 + p) * 2 + (take & 1)];
-                }
-                const int missing = *(volatile int*)&s_missing[j & 7];
-                if (missing != 0 || key0 + kN > seq_len) {          // keys behind the last one and of no page: their weights are zero
+                Codes x = next;
+                if (j + 1 < most) next = load(j + 1);
+                if (key0 + kN > seq_len) {                          // keys behind the last one: so are theirs
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
                         const int key = key0 + octet * 8 + 2 * p;
-                        const uint32_t keep = (missing >> (octet >> 1)) & 1 ? 0u : (key < seq_len ? 0xffffu : 0u) | (key + 1 < seq_len ? 0xffff0000u : 0u);
+                        const uint32_t keep = (key < seq_len ? 0xffffu : 0u) | (key + 1 < seq_len ? 0xffff0000u : 0u);
 #pragma unroll
-                        for (int k = 0; k < HG; ++k) vw[p].w[k] &= keep;
+                        for (int k = 0; k < HG; ++k) x.w[p].w[k] &= keep;
                     }
                 }
                 uint32_t odd = 0;                                   // a sign bit is set where a word is not a number
 #pragma unroll
                 for (int p = 0; p < 4; ++p)
 #pragma unroll
-                    for (int k = 0; k < HG; ++k) odd |= (vw[p].w[k] & 0x7f807f80u) + 0x00800080u;
+                    for (int k = 0; k < HG; ++k) odd |= (x.w[p].w[k] & 0x7f807f80u) + 0x00800080u;
                 if (odd & 0x80008000u) {
                     atomicExch(&s_odd, 1);
 #pragma unroll
                     for (int p = 0; p < 4; ++p)
 #pragma unroll
                         for (int k = 0; k < HG; ++k) {
-                            const uint32_t at = ((vw[p].w[k] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-                            vw[p].w[k] &= (at & 0x8000u ? 0u : 0xffffu) | (at & 0x80000000u ? 0u : 0xffff0000u);
+                            const uint32_t at = ((x.w[p].w[k] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+                            x.w[p].w[k] &= (at & 0x8000u ? 0u : 0xffffu) | (at & 0x80000000u ? 0u : 0xffff0000u);
                         }
                 }
                 if (!free_again(pv_done, j, 57)) break;
@@ -423,12 +435,12 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
                     uint32_t v[4][4];                               // [column][pair of keys]
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
-                        const uint32_t w = vw[p].w[k], zero = mul_bf16x2(w & 0x000f000fu, kMinus2p127), step = mul_bf16x2(w & 0xfff0fff0u, k64);
-                        const uint32_t x = vc[p].w[k], y = x >> 8;
-                        v[0][p] = mul_bf16x2(fma_bf16x2(x & 0x000f000fu, k2p127, zero), step);
-                        v[1][p] = mul_bf16x2(fma_bf16x2(x & 0x00f000f0u, k2p123, zero), step);
-                        v[2][p] = mul_bf16x2(fma_bf16x2(y & 0x000f000fu, k2p127, zero), step);
-                        v[3][p] = mul_bf16x2(fma_bf16x2(y & 0x00f000f0u, k2p123, zero), step);
+                        const uint32_t w = x.w[p].w[k], zero = mul_bf16x2(w & 0x000f000fu, kMinus2p127), step = mul_bf16x2(w & 0xfff0fff0u, k64);
+                        const uint32_t lo = x.c[p].w[k], hi = lo >> 8;
+                        v[0][p] = mul_bf16x2(fma_bf16x2(lo & 0x000f000fu, k2p127, zero), step);
+                        v[1][p] = mul_bf16x2(fma_bf16x2(lo & 0x00f000f0u, k2p123, zero), step);
+                        v[2][p] = mul_bf16x2(fma_bf16x2(hi & 0x000f000fu, k2p127, zero), step);
+                        v[3][p] = mul_bf16x2(fma_bf16x2(hi & 0x00f000f0u, k2p123, zero), step);
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -438,11 +450,12 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&v_full[b]), mbar_arrive(&raw_free[j % kRawStages]);
+                if (lane == 0) mbar_arrive(&v_full[b]);
             }
         }
     } else if (active && warp < kSoftWarps) {
         // ---- softmax: a thread per row (TMEM lane 32 * (warp % 4) + lane) ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         const int t = warp >> 2;
         const int my_tiles = tiles[t];
         const int row_local = tid & 127;
@@ -458,7 +471,7 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             ok = wait_all(&s_full[t * 2 + b], (uint32_t)((j >> 1) & 1), 59);
             if (!ok) break;
             tcgen05_fence_after();
-            const int missing = *(volatile int*)&s_missing[j & 7];
+            const int missing = *(volatile int*)&s_missing[j & 3];
             const bool need_mask = key0 + kN - 1 > pos || window > 0 || missing != 0;
             const int hi = pos - key0;                              // columns <= hi are visible ...
             const int lo = window > 0 ? hi - window : -1;           // ... and > lo
@@ -471,34 +484,54 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
                 for (int e = 0; e < kN; ++e)
                     if (!(e <= hi && e > lo) || ((missing >> (e / kBlock)) & 1)) v[e / 32][e % 32] = __float_as_uint(-INFINITY);
             }
+            // P = 2^(s * scale - m), two at a time: a packed multiply-add, two ex2, a packed addition and a conversion.  From the fifth tile on m is
+            // taken as it is and the tile's maximum found meanwhile; where it is more than 8 above m, the weights are computed again.
             float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            auto largest = [&]() {
 #pragma unroll
-            for (int e = 0; e < kN; e += 2)
-                part[(e >> 1) & 3] = max3(part[(e >> 1) & 3], __uint_as_float(v[e / 32][e % 32]), __uint_as_float(v[e / 32][e % 32 + 1]));
-            const float mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * scale_log2;
+                for (int e = 0; e < kN; e += 2)
+                    part[(e >> 1) & 3] = max3(part[(e >> 1) & 3], __uint_as_float(v[e / 32][e % 32]), __uint_as_float(v[e / 32][e % 32 + 1]));
+                return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * scale_log2;
+            };
             float corr = 1.f;
             bool rescale = false;
-            if (mx > m_used + (j < 256 / kN ? 0.f : 8.f) || (m_used == -INFINITY && mx != -INFINITY)) {
-                corr = m_used == -INFINITY ? 0.f : exp2f(m_used - mx);
-                m_used = mx;
-                l *= corr;
-                rescale = j > 0;
-            }
-            const float m_eff = m_used == -INFINITY ? 0.f : m_used;
-            // P = 2^(s * scale - m), two at a time: a packed multiply-add, two ex2, a packed addition and a conversion
-            const uint64_t scale2 = pack2(scale_log2, scale_log2), minus_m = pack2(-m_eff, -m_eff);
+            auto raise = [&](float mx, float by) {
+                if (mx > m_used + by || (m_used == -INFINITY && mx != -INFINITY)) {
+                    corr = m_used == -INFINITY ? 0.f : exp2f(m_used - mx);
+                    m_used = mx;
+                    l *= corr;
+                    rescale = j > 0;
+                }
+            };
+            const uint64_t scale2 = pack2(scale_log2, scale_log2);
             uint32_t p[32];
-            uint64_t sums[2] = {0, 0};
+            float2 sum;
+            auto weights = [&]() {
+                const float m_eff = m_used == -INFINITY ? 0.f : m_used;
+                const uint64_t minus_m = pack2(-m_eff, -m_eff);
+                uint64_t sums[2] = {0, 0};
 #pragma unroll
-            for (int e = 0; e < kN; e += 2) {
-                const float2 x = unpack2(fma2(pack2(__uint_as_float(v[e / 32][e % 32]), __uint_as_float(v[e / 32][e % 32 + 1])), scale2, minus_m));
-                float2 y;
-                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(x.x));
-                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(x.y));
-                sums[(e >> 1) & 1] = add2(sums[(e >> 1) & 1], pack2(y.x, y.y));
-                p[e / 2] = pack_bf16(y.x, y.y);
+                for (int e = 0; e < kN; e += 2) {
+                    const float2 x = unpack2(fma2(pack2(__uint_as_float(v[e / 32][e % 32]), __uint_as_float(v[e / 32][e % 32 + 1])), scale2, minus_m));
+                    float2 y;
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(x.x));
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(x.y));
+                    sums[(e >> 1) & 1] = add2(sums[(e >> 1) & 1], pack2(y.x, y.y));
+                    p[e / 2] = pack_bf16(y.x, y.y);
+                }
+                sum = unpack2(add2(sums[0], sums[1]));
+            };
+            if (j < 256 / kN) {
+                raise(largest(), 0.f);
+                weights();
+            } else {
+                weights();
+                const float mx = largest();
+                if (__any_sync(0xffffffffu, mx > m_used + 8.f || (m_used == -INFINITY && mx != -INFINITY))) {
+                    raise(mx, 8.f);
+                    weights();
+                }
             }
-            const float2 sum = unpack2(add2(sums[0], sums[1]));
             l += sum.x + sum.y;
             if (j > 0 && __any_sync(0xffffffffu, rescale)) {
                 ok = wait_all(&pv_done[t * 2 + (b ^ 1)], (uint32_t)(((j - 1) >> 1) & 1), 60);
@@ -582,6 +615,13 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kTmemCols) : "memory");
 }
 
+// The registers that a launch gives a thread: the split among the warps counts on them.
+template <typename Kernel>
+static int launch_registers(Kernel kernel) {
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : -1;
+}
+
 }  // namespace kv4p
 }  // namespace cib
 
@@ -607,6 +647,8 @@ extern "C" int cib_attention_kv4_prompt(const void* q, int q_stride, void* out, 
     if (d == DV) {                                                                                                                                  \
         static SmemLimit limit;                                                                                                                     \
         if (int rc = raise_smem_limit(limit, kv4p::attention_prompt_kernel<DV>, kv4p::Smem<DV>::kTotal, "attention_kv4_prompt")) return rc;         \
+        static const int regs = kv4p::launch_registers(kv4p::attention_prompt_kernel<DV>);                                                          \
+        CIB_REQUIRE(regs == kv4p::kLaunchRegs, "attention_kv4_prompt: built with %d registers a thread, laid out for %d", regs, kv4p::kLaunchRegs); \
         const cudaError_t e = launch_pdl(kv4p::attention_prompt_kernel<DV>, dim3(nkv, num_pairs), dim3(kv4p::kThreads), (size_t)kv4p::Smem<DV>::kTotal, \
                                          stream, prompt_pdl(), (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride,                  \
                                          (const unsigned char*)cache, num_pages, page_size, block_table, table_stride, query_start_loc, seq_lens,   \
