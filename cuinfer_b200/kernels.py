@@ -780,10 +780,11 @@ def kv4_cache_shape(num_pages: int, num_kv_heads: int, page_size: int, head_dim:
 
 def _kv4_cache(cache: torch.Tensor, num_kv_heads: int, head_dim: int, who: str) -> int:
     """Checks the cache; its page size."""
-    if cache.dtype != torch.uint8 or cache.dim() != 4 or cache.shape[1] != num_kv_heads or cache.shape[3] != 18 * head_dim:
+    shape = cache.shape
+    if cache.dtype is not torch.uint8 or len(shape) != 4 or shape[1] != num_kv_heads or shape[3] != 18 * head_dim:
         raise KernelError(f"{who}: cache must be uint8 [pages, {num_kv_heads}, page_size / {KV4_BLOCK}, {18 * head_dim}], got "
-                          f"{cache.dtype} {list(cache.shape)}")
-    return cache.shape[2] * KV4_BLOCK
+                          f"{cache.dtype} {list(shape)}")
+    return shape[2] * KV4_BLOCK
 
 
 def _same_device(who: str, *tensors) -> None:
@@ -795,10 +796,20 @@ def _same_device(who: str, *tensors) -> None:
         index = t.get_device()
         if index < 0:
             raise KernelError(f"{who}: every tensor must be a CUDA tensor; cuinfer_b200 has no CPU path")
-        if here < 0:
-            here = torch.cuda.current_device()
         if index != here:
-            raise KernelError(f"{who}: every tensor must be on the current device (cuda:{here}), got cuda:{index}")
+            if here < 0:
+                here = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+            if index != here:
+                raise KernelError(f"{who}: every tensor must be on the current device (cuda:{here}), got cuda:{index}")
+
+
+def _dense(t: torch.Tensor, what: str, dtype: torch.dtype | None = None) -> int:
+    """The address of a contiguous tensor that ``_same_device`` has seen (a decode step's calls are as long as their checks)."""
+    if dtype is not None and t.dtype is not dtype:
+        raise KernelError(f"{what} must be {dtype}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise KernelError(f"{what} must be contiguous")
+    return t.data_ptr()
 
 
 def qk_norm_rope_kv4_write(qkv: torch.Tensor, positions: torch.Tensor, slot_mapping: torch.Tensor, q_weight: torch.Tensor | None,
@@ -812,18 +823,18 @@ def qk_norm_rope_kv4_write(qkv: torch.Tensor, positions: torch.Tensor, slot_mapp
     who = "qk_norm_rope_kv4_write"
     if qkv.dim() != 2 or qkv.stride(1) != 1:
         raise KernelError(f"{who}: qkv must be [T, (nq + 2 nkv) * d] with dense rows")
-    T = qkv.shape[0]
-    if qkv.shape[1] < (num_q_heads + 2 * num_kv_heads) * head_dim:
-        raise KernelError(f"{who}: qkv rows of {qkv.shape[1]} values do not hold {num_q_heads} + 2 x {num_kv_heads} heads of {head_dim}")
+    T, width = qkv.shape
+    if width < (num_q_heads + 2 * num_kv_heads) * head_dim:
+        raise KernelError(f"{who}: qkv rows of {width} values do not hold {num_q_heads} + 2 x {num_kv_heads} heads of {head_dim}")
     page_size = _kv4_cache(cache, num_kv_heads, head_dim, who)
     if q_out is None:
         q_out = qkv
-    elif q_out.shape != (T, num_q_heads * head_dim) or q_out.dtype != qkv.dtype or q_out.stride(1) != 1:
+    elif q_out.shape != (T, num_q_heads * head_dim) or q_out.dtype is not qkv.dtype or q_out.stride(1) != 1:
         raise KernelError(f"{who}: q_out must be {qkv.dtype} [{T}, {num_q_heads * head_dim}] with dense rows")
     if positions.numel() < T or slot_mapping.numel() < T:
         raise KernelError(f"{who}: a position and a slot for each of the {T} tokens")
     has_norm = q_weight is not None
-    if (k_weight is not None) != has_norm or (has_norm and q_weight.dtype != k_weight.dtype):
+    if (k_weight is not None) != has_norm or (has_norm and q_weight.dtype is not k_weight.dtype):
         raise KernelError(f"{who}: q and k norm weights must both be given, in one dtype")
     if has_norm and (q_weight.numel() != head_dim or k_weight.numel() != head_dim):
         raise KernelError(f"{who}: norm weights must have {head_dim} elements")
@@ -831,20 +842,21 @@ def qk_norm_rope_kv4_write(qkv: torch.Tensor, positions: torch.Tensor, slot_mapp
         raise KernelError(f"{who}: rope table must be [positions, {rotary_dim // 2}, 2], got {list(rope_table.shape)}")
     _same_device(who, qkv, cache, q_out, positions, slot_mapping, q_weight, k_weight, rope_table)
     rc = library().cib_qk_norm_rope_kv4_write(
-        _cuda(qkv, "qkv", contiguous=False), _code(qkv, "qkv"), _row_stride(qkv), _cuda(q_out, "q_out", contiguous=False), _row_stride(q_out),
-        _cuda(positions, "positions", torch.int32), _cuda(slot_mapping, "slot_mapping", torch.int32),
-        _cuda(q_weight, "q_weight") if has_norm else None, _cuda(k_weight, "k_weight") if has_norm else None,
-        _code(q_weight, "q_weight") if has_norm else 0, 1 if has_norm else 0, float(eps),
-        _cuda(rope_table, "rope_table", torch.float32) if rope_table is not None else None,
+        qkv.data_ptr(), _code(qkv, "qkv"), _row_stride(qkv), q_out.data_ptr(), _row_stride(q_out),
+        _dense(positions, "positions", torch.int32), _dense(slot_mapping, "slot_mapping", torch.int32),
+        _dense(q_weight, "q_weight") if has_norm else None, _dense(k_weight, "k_weight") if has_norm else None,
+        _code(q_weight, "q_weight") if has_norm else 0, 1 if has_norm else 0, eps,
+        _dense(rope_table, "rope_table", torch.float32) if rope_table is not None else None,
         rotary_dim if rope_table is not None else 0, rope_table.shape[0] if rope_table is not None else 0,
-        _cuda(cache, "cache"), cache.shape[0], page_size, T, num_q_heads, num_kv_heads, head_dim, 1 if use_pdl else 0, _stream())
+        _dense(cache, "cache"), cache.shape[0], page_size, T, num_q_heads, num_kv_heads, head_dim, 1 if use_pdl else 0, _stream())
     _check(rc, who)
     _count()
 
 
 def _row_stride(t: torch.Tensor) -> int:
     """Elements from a row to the next (of a single row: its length, whatever torch calls its stride)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    rows, width = t.shape
+    return t.stride(0) if rows > 1 else max(t.stride(0), width)
 
 
 def kv4_read(cache: torch.Tensor, slots: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, num_kv_heads: int, head_dim: int) -> None:
@@ -857,9 +869,8 @@ def kv4_read(cache: torch.Tensor, slots: torch.Tensor, keys: torch.Tensor, value
         if t.shape != (T, width) or t.dtype != keys.dtype or t.stride(1) != 1:
             raise KernelError(f"{who}: {name} must be {keys.dtype} [{T}, {width}] with dense rows")
     _same_device(who, cache, slots, keys, values)
-    rc = library().cib_kv4_read(_cuda(cache, "cache"), cache.shape[0], page_size, _cuda(slots, "slots", torch.int32),
-                                _cuda(keys, "keys", contiguous=False), _row_stride(keys), _cuda(values, "values", contiguous=False),
-                                _row_stride(values), _code(keys, "keys"), T, num_kv_heads, head_dim, 1 if use_pdl else 0, _stream())
+    rc = library().cib_kv4_read(_dense(cache, "cache"), cache.shape[0], page_size, _dense(slots, "slots", torch.int32),
+                                keys.data_ptr(), _row_stride(keys), values.data_ptr(), _row_stride(values), _code(keys, "keys"), T, num_kv_heads, head_dim, 1 if use_pdl else 0, _stream())
     _check(rc, who)
     _count()
 
@@ -888,21 +899,24 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
         raise KernelError(f"{who}: block_table rows must be dense")
     if window < 0 or max_seq_len < 0:
         raise KernelError(f"{who}: window and max_seq_len must not be negative")
+    if block_table.dtype is not torch.int32:
+        raise KernelError(f"{who}: block_table must be torch.int32, got {block_table.dtype}")
     _same_device(who, q, out, cache, block_table, query_start_loc, seq_lens)
     if T == 0 or R == 0:
         return
-    cache_args = (_cuda(cache, "cache"), cache.shape[0], page_size, _cuda(block_table, "block_table", torch.int32, contiguous=False),
-                  _row_stride(block_table), _cuda(query_start_loc, "query_start_loc", torch.int32), _cuda(seq_lens, "seq_lens", torch.int32))
-    q_args = (_cuda(q, "q", contiguous=False), _row_stride(q))
-    out_args = (_cuda(out, "out", contiguous=False), _row_stride(out))
+    lib = library()
+    cache_args = (_dense(cache, "cache"), cache.shape[0], page_size, block_table.data_ptr(), _row_stride(block_table),
+                  _dense(query_start_loc, "query_start_loc", torch.int32), _dense(seq_lens, "seq_lens", torch.int32))
+    q_args = (q.data_ptr(), _row_stride(q))
+    out_args = (out.data_ptr(), _row_stride(out))
     dtype = _code(q, "q")
     pdl = 1 if use_pdl else 0
+    bound = sum(query_lens_host) > T
     least_query = 1
     # Single tokens run on the kernel that splits keys; the lengths are a bound where they name more rows than there are, and any
     # request may then bring a single token.
-    if (dtype == BF16 and library().cib_attention_kv4_decode_supports(head_dim, page_size) and q_args[1] % 8 == 0 and q_args[0] % 16 == 0
-            and (1 in query_lens_host or sum(query_lens_host) > T)):
-        lib = library()
+    if (dtype == BF16 and (bound or 1 in query_lens_host) and lib.cib_attention_kv4_decode_supports(head_dim, page_size) and q_args[1] % 8 == 0
+            and q_args[0] % 16 == 0):
         ctas, unit = kv4_decode_shape(R * num_kv_heads * -(-(num_q_heads // num_kv_heads) // 8), min(max_seq_len, window + 16 if window else max_seq_len),
                                       lib.cib_attention_kv4_decode_ctas(head_dim))
         scratch = None
@@ -913,25 +927,25 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
         _check(rc, who)
         note_flagged_launch()
         _count()
-        if T <= R and max(query_lens_host) <= 1:
+        if T <= R and max(query_lens_host) <= 1:                # (nothing but single tokens)
             return
         least_query = 2
-    if (dtype == BF16 and library().cib_attention_kv4_prompt_supports(head_dim, page_size) and scale > 0
+    if (dtype == BF16 and lib.cib_attention_kv4_prompt_supports(head_dim, page_size) and scale > 0
             and q_args[1] % 8 == 0 and q_args[0] % 16 == 0 and out_args[1] % 8 == 0 and out_args[0] % 16 == 0):
         g = num_q_heads // num_kv_heads
-        if sum(query_lens_host) > T:
+        if bound:
             pairs = T * g // 256 + R
         else:
             pairs = sum(-(-n * g // 256) for n in query_lens_host if n >= least_query)
         folded = window <= 0 and pairs * num_kv_heads <= 148
-        rc = library().cib_attention_kv4_prompt(*q_args, *out_args, *cache_args, R, pairs, 1 if folded else 0, least_query, num_q_heads, num_kv_heads,
-                                                head_dim, float(scale), int(window), _error_flag(q.device).data_ptr(), _stream())
+        rc = lib.cib_attention_kv4_prompt(*q_args, *out_args, *cache_args, R, pairs, 1 if folded else 0, least_query, num_q_heads, num_kv_heads,
+                                         head_dim, float(scale), int(window), _error_flag(q.device).data_ptr(), _stream())
         _check(rc, who)
         note_flagged_launch()
         _count()
         return
-    rc = library().cib_attention_kv4_generic(q_args[0], dtype, q_args[1], *out_args, *cache_args, T, R, max_seq_len, least_query, num_q_heads, num_kv_heads,
-                                             head_dim, float(scale), int(window), pdl, _stream())
+    rc = lib.cib_attention_kv4_generic(q_args[0], dtype, q_args[1], *out_args, *cache_args, T, R, max_seq_len, least_query, num_q_heads, num_kv_heads,
+                                       head_dim, float(scale), int(window), pdl, _stream())
     _check(rc, who)
     _count()
 
