@@ -20,7 +20,11 @@
 //
 // A running maximum and sum per head in base 2, in 32 bits; the warps of a CTA are merged in shared memory.
 //
-// The work of a launch is one list: the blocks of request 0, head block 0, then head block 1, .. , request 1, .., in units of `unit`
+// Few (request, head block)s of moderate length: a cluster of up to eight CTAs shares the blocks of each, the partial results stay in the CTAs' shared memory
+// and every CTA reads its share of the columns from all of them (distributed shared memory).  No list, no scratch, no second kernel: 8 requests of
+// 4 096 tokens took 18.4 + 7.4 us with those, 18.8 so; one of 300 10.7 in one CTA a head, 7.8 so.
+//
+// Else the work of a launch is one list: the blocks of request 0, head block 0, then head block 1, .. , request 1, .., in units of `unit`
 // blocks.  The launch has as many CTAs as the GPU holds at once and every CTA takes the same number of consecutive units, found from the
 // lengths on the device: requests of any lengths end together, and a recorded launch fits whatever lengths it is replayed with.
 // What a CTA has of a (request, head block) goes straight to the output if it is all of it; else it is a partial result: its first or its
@@ -31,11 +35,14 @@
 #include "mma_utils.cuh"
 #include "tcgen05_utils.cuh"
 
+#include <cooperative_groups.h>
+
 namespace cib {
 namespace kv4 {
 
 constexpr int kDecWarps = 4;
 constexpr int kDecStages = 3;
+constexpr int kDecCluster = 8;       // CTAs that share a (request, head block), at most
 constexpr int kDecHeads = 8;         // query heads of a CTA: the columns of an MMA
 
 template <int D>
@@ -132,7 +139,8 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                  ::"r"(tc_smem_u32(dst)), "l"(src), "r"(bytes), "r"(tc_smem_u32(bar)) : "memory");
 }
 
-template <int D>
+// CLUSTER: gridDim.x CTAs, one cluster, for each (request, head block) blockIdx.y; else the list.
+template <int D, bool CLUSTER>
 __global__ void __launch_bounds__(kDecWarps * 32, D > 128 ? 2 : 4)
 attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* __restrict__ out, int out_stride,
                         const unsigned char* __restrict__ cache, int num_pages, int page_size, const int* __restrict__ block_table, int table_stride,
@@ -149,41 +157,59 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
 
     if (lane < kDecStages) mbar_init(&s_full[warp * kDecStages + lane], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (warp == 0) {
+    if (threadIdx.x == 0) s_failed = 0;
+    if (!CLUSTER && warp == 0) {
         const Place p = warp_find(blockIdx.x, gridDim.x, num_requests, query_start_loc, seq_lens, window, unit, head_blocks);
-        if (lane == 0) s_place = p, s_failed = 0;
+        if (lane == 0) s_place = p;
     }
     __syncthreads();
     griddep_wait();          // queries and this step's keys and values come from the kernel before
     griddep_launch();
-    const Place place = s_place;
-    const long long share = (place.total + gridDim.x - 1) / gridDim.x;
-    const long long from = blockIdx.x * share, to = min(place.total, from + share);
     const int per_page = page_size / kBlock;
     unsigned char* ring = smem + warp * kDecStages * stage_bytes<D>();
     uint64_t* full = s_full + warp * kDecStages;
     int st = 0;                      // the ring stage that is read next, and the parity of its barrier
     uint32_t parity = 0;
-    long long before = place.before, at = from;
-    int r = place.request;
+    long long share = 0, to = 1, before = 0, at = 0;
+    int r = CLUSTER ? (int)blockIdx.y / head_blocks : 0;
+    if (!CLUSTER) {
+        const Place place = s_place;
+        share = (place.total + gridDim.x - 1) / gridDim.x;
+        at = blockIdx.x * share, to = min(place.total, at + share);
+        before = place.before, r = place.request;
+    }
+    const long long from = at;
 
     while (at < to) {
-    int units = units_of(r, query_start_loc, seq_lens, window, unit);
-    while (at >= before + (long long)units * head_blocks) {
-        before += (long long)units * head_blocks;
-        units = units_of(++r, query_start_loc, seq_lens, window, unit);
+    int hblock, u0, u1, step = unit;                              // units of `step` blocks
+    bool first_piece = true, alone = true;
+    if constexpr (CLUSTER) {
+        if (query_start_loc[r + 1] - query_start_loc[r] != 1) return;          // (the whole cluster)
+        hblock = (int)blockIdx.y - r * head_blocks;
+        // equal shares in steps of two blocks, and two for every warp at least
+        const int blocks = span_of(seq_lens[r], window).count, mine = (blocks + (int)gridDim.x - 1) / (int)gridDim.x;
+        step = max(2 * kDecWarps, (mine + 1) / 2 * 2);
+        u0 = min((int)blockIdx.x, (blocks + step - 1) / step), u1 = u0 + 1;
+        at = to;
+    } else {
+        int units = units_of(r, query_start_loc, seq_lens, window, unit);
+        while (at >= before + (long long)units * head_blocks) {
+            before += (long long)units * head_blocks;
+            units = units_of(++r, query_start_loc, seq_lens, window, unit);
+        }
+        const int local = (int)(at - before);
+        hblock = local / units, u0 = local - hblock * units;
+        u1 = (int)min((long long)units, u0 + (to - at));
+        first_piece = at == from;
+        at += u1 - u0;
+        alone = u0 == 0 && u1 == units;
     }
-    const int local = (int)(at - before), hblock = local / units, u0 = local - hblock * units;
-    const int u1 = (int)min((long long)units, u0 + (to - at));
-    const bool first_piece = at == from;
-    at += u1 - u0;
-    const bool alone = u0 == 0 && u1 == units;
     const int kvh = hblock / blocks_per_kv, hb = hblock - kvh * blocks_per_kv;
     const int head0 = kvh * g + hb * kDecHeads, nh = min(kDecHeads, g - hb * kDecHeads);
     const int token = query_start_loc[r];
     const int seq_len = seq_lens[r];
     const Span span = span_of(seq_len, window);
-    const int begin = span.first + u0 * unit, end = span.first + min(span.count, u1 * unit);
+    const int begin = span.first + min(span.count, u0 * step), end = span.first + min(span.count, u1 * step);
     const int lo = window > 0 ? max(0, seq_len - window) : 0;
     const int* table = block_table + (size_t)r * table_stride;
 
@@ -454,6 +480,7 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
         for (int k = 0; k < NG; ++k) dst[k * 8] = make_float4(o[2 * k][e], o[2 * k][2 + e], o[2 * k + 1][e], o[2 * k + 1][2 + e]);
     }
     __syncthreads();
+    float* sm_part = sm_l + kDecWarps * kDecHeads;                // a cluster's CTA: [head][D] values, [head][2] maximum and sum
     for (int i = threadIdx.x; i < nh * D; i += kDecWarps * 32) {
         const int h = i / D, x = i - h * D;
         float M = -INFINITY, L = 0.f, O = 0.f;
@@ -466,7 +493,10 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             O += sm_o[(size_t)(w * kDecHeads + h) * D + x] * f;
         }
         O *= 64.f;                              // (the operands were (code - zero) 2^-6)
-        if (alone) {
+        if (CLUSTER && gridDim.x > 1) {
+            sm_part[i] = O;
+            if (x == 0) sm_part[kDecHeads * D + h * 2] = M, sm_part[kDecHeads * D + h * 2 + 1] = L;
+        } else if (alone) {
             out[(size_t)token * out_stride + (size_t)(head0 + h) * D + x] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L);
         } else {
             const size_t place = ((size_t)blockIdx.x * 2 + (first_piece ? 0 : 1)) * kDecHeads + h;
@@ -474,17 +504,43 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             if (x == 0) part_ml[place * 2] = M, part_ml[place * 2 + 1] = L;
         }
     }
+    if (CLUSTER && gridDim.x > 1) {
+        namespace cg = cooperative_groups;
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();                                           // every CTA's part is in its shared memory
+        for (int i = (int)blockIdx.x * kDecWarps * 32 + threadIdx.x; i < nh * D; i += (int)gridDim.x * kDecWarps * 32) {
+            const int h = i / D;
+            float m[kDecCluster], M = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll
+            for (int c = 0; c < kDecCluster; ++c) {
+                m[c] = c < (int)gridDim.x ? cluster.map_shared_rank(sm_part, c)[kDecHeads * D + h * 2] : -INFINITY;
+                M = fmaxf(M, m[c]);
+            }
+#pragma unroll
+            for (int c = 0; c < kDecCluster; ++c) {
+                if (c >= (int)gridDim.x) break;
+                const float* part = cluster.map_shared_rank(sm_part, c);
+                const float f = m[c] == -INFINITY ? 0.f : ex2(m[c] - M);
+                L += part[kDecHeads * D + h * 2 + 1] * f;
+                O += part[i] * f;
+            }
+            out[(size_t)token * out_stride + (size_t)head0 * D + i] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L);
+        }
+        cluster.sync();                                           // (a CTA's shared memory has been read before it leaves)
+    }
     __syncthreads();     // (the rings are filled again)
     }
 }
 
-// A CTA per (head, request), a thread per value: joins what several CTAs have of it.
+// A CTA per (head, request), a thread per value: joins what several CTAs have of it.  The maxima and sums of up to D parts are fetched at once, a
+// part a thread; the values then eight parts at a time (part after part, each a trip to the L2, took 13 us for 20 parts).
 template <int D>
 __global__ void __launch_bounds__(D)
 attention_decode_merge_kernel(__nv_bfloat16* __restrict__ out, int out_stride, const int* __restrict__ query_start_loc, const int* __restrict__ seq_lens,
                               int num_requests, int nq, int nkv, int window, int unit, int parts, const float* __restrict__ part_o,
                               const float* __restrict__ part_ml) {
     __shared__ long long s_total[2];
+    __shared__ float s_weight[D], s_warp[2][D / 32];
     const int head = blockIdx.x, r = blockIdx.y, x = threadIdx.x;
     const int g = nq / nkv, blocks_per_kv = (g + kDecHeads - 1) / kDecHeads, head_blocks = nkv * blocks_per_kv;
     if (threadIdx.x < 32) {
@@ -513,14 +569,31 @@ attention_decode_merge_kernel(__nv_bfloat16* __restrict__ out, int out_stride, c
     // the first CTA has it as its last piece, unless it is also its first; all others as their first
     auto place_of = [&](int c) { return ((size_t)c * 2 + (c == c0 && from != c0 * share ? 1 : 0)) * kDecHeads + h; };
     float M = -INFINITY, L = 0.f, O = 0.f;
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) M = fmaxf(M, part_ml[place_of(c) * 2]);
+    for (int first = c0; first <= c1; first += D) {
+        const int count = min(D, c1 + 1 - first);
+        float m = -INFINITY, l = 0.f;
+        if (x < count) {
+            const float2 ml = *reinterpret_cast<const float2*>(part_ml + place_of(first + x) * 2);
+            m = ml.x, l = ml.y;
+        }
+        const float top = warp_max(m);
+        if ((x & 31) == 0) s_warp[0][x >> 5] = top;
+        __syncthreads();
+        float here = M;
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) here = fmaxf(here, s_warp[0][w]);
+        const float f = m == -INFINITY ? 0.f : ex2(m - here);
+        s_weight[x] = f;
+        const float sum = warp_sum(l * f);
+        if ((x & 31) == 0) s_warp[1][x >> 5] = sum;
+        __syncthreads();
+        const float keep = M == -INFINITY ? 0.f : ex2(M - here);
+        M = here, L *= keep, O *= keep;
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) L += s_warp[1][w];
 #pragma unroll 8
-    for (int c = c0; c <= c1; ++c) {
-        const size_t place = place_of(c);
-        const float m = part_ml[place * 2], f = m == -INFINITY ? 0.f : ex2(m - M);
-        L += part_ml[place * 2 + 1] * f;
-        O += part_o[place * D + x] * f;
+        for (int c = 0; c < count; ++c) O += part_o[place_of(first + c) * D + x] * s_weight[c];
+        __syncthreads();
     }
     out[(size_t)query_start_loc[r] * out_stride + (size_t)head * D + x] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L);
 }
@@ -538,16 +611,18 @@ extern "C" int cib_attention_kv4_decode_supports(int d, int page_size) {
 extern "C" int cib_attention_kv4_decode_ctas(int d) { return 148 * (d > 128 ? 2 : 4); }
 extern "C" long long cib_attention_kv4_decode_scratch_floats(int d, int ctas) { return (long long)ctas * 2 * kv4::kDecHeads * (d + 2); }
 
-// Computes the rows of the requests that bring one token; the others' are left as they are.  ctas: how many CTAs share the work; unit: blocks
+// Computes the rows of the requests that bring one token; the others' are left as they are.  cluster > 0: so many CTAs (1, 2, 4 or 8) share the blocks of
+// each (request, head block); ctas, unit and scratch mean nothing then.  Else ctas: how many CTAs share the work; unit: blocks
 // of 16 keys that a CTA has at least.  scratch: cib_attention_kv4_decode_scratch_floats, or none where no request has more than `unit`
 // blocks (no request is split then, whatever its length).
 extern "C" int cib_attention_kv4_decode(const void* q, int q_stride, void* out, int out_stride, const void* cache, int num_pages, int page_size,
                                         const int* block_table, int table_stride, const int* query_start_loc, const int* seq_lens, int num_requests, int nq,
-                                        int nkv, int d, float scale, int window, int ctas, int unit, float* scratch, int* error_flag, int use_pdl,
+                                        int nkv, int d, float scale, int window, int cluster, int ctas, int unit, float* scratch, int* error_flag, int use_pdl,
                                         cudaStream_t stream) {
     CIB_REQUIRE(cib_attention_kv4_decode_supports(d, page_size), "attention_kv4_decode: head size %d (64, 128 or 256), page size %d (a multiple of 16) are not taken", d, page_size);
     CIB_REQUIRE(num_requests >= 0 && num_requests <= 65535 && nq > 0 && nkv > 0 && nq % nkv == 0, "attention_kv4_decode: bad sizes R=%d nq=%d nkv=%d", num_requests, nq, nkv);
-    CIB_REQUIRE(ctas >= 1 && unit >= 1 && unit <= 1 << 20, "attention_kv4_decode: bad launch shape %d, %d", ctas, unit);
+    CIB_REQUIRE(cluster == 0 || cluster == 1 || cluster == 2 || cluster == 4 || cluster == kv4::kDecCluster, "attention_kv4_decode: clusters of 1, 2, 4 or 8, not %d", cluster);
+    CIB_REQUIRE(cluster > 0 || (ctas >= 1 && (scratch == nullptr || (unit >= 1 && unit <= 1 << 20))), "attention_kv4_decode: bad launch shape %d, %d", ctas, unit);
     CIB_REQUIRE(num_pages > 0 && table_stride > 0 && cache != nullptr && ((uintptr_t)cache % 16) == 0, "attention_kv4_decode: bad cache geometry");
     CIB_REQUIRE((long long)num_pages * nkv * (page_size / kv4::kBlock) < (1ll << 31), "attention_kv4_decode: more than 2^31 blocks");
     CIB_REQUIRE(q_stride % 8 == 0 && ((uintptr_t)q % 16) == 0, "attention_kv4_decode: query rows must be 16-byte aligned");
@@ -555,15 +630,28 @@ extern "C" int cib_attention_kv4_decode(const void* q, int q_stride, void* out, 
     if (num_requests == 0) return 0;
     const float scale_log2 = scale * 1.4426950408889634f;
     if (scratch == nullptr) unit = 1 << 27;          // a request is one unit, so no CTA has a part of it
+    const long long pairs = (long long)num_requests * nkv * ((nq / nkv + kv4::kDecHeads - 1) / kv4::kDecHeads);
+    CIB_REQUIRE(cluster == 0 || pairs <= 65535, "attention_kv4_decode: %lld (request, head block)s are too many for clusters", pairs);
     float* part_ml = scratch == nullptr ? nullptr : scratch + (size_t)ctas * 2 * kv4::kDecHeads * d;
 #define CIB_KV4_DECODE(DV)                                                                                                                           \
+    if (d == DV && cluster > 0) {                                                                                                                    \
+        static SmemLimit limit;                                                                                                                      \
+        if (int rc = raise_smem_limit(limit, kv4::attention_decode_kernel<DV, true>, kv4::ring_bytes<DV>(), "attention_kv4_decode")) return rc;      \
+        const cudaError_t e = launch_pdl_cluster(kv4::attention_decode_kernel<DV, true>, dim3(cluster, (unsigned)pairs), dim3(kv4::kDecWarps * 32),  \
+                                                 (size_t)kv4::ring_bytes<DV>(), stream, use_pdl != 0, cluster, (const __nv_bfloat16*)q, q_stride,    \
+                                                 (__nv_bfloat16*)out, out_stride, (const unsigned char*)cache, num_pages, page_size, block_table,    \
+                                                 table_stride, query_start_loc, seq_lens, num_requests, nq, nkv, scale_log2, window, 1,              \
+                                                 nullptr, nullptr, error_flag);                                                                      \
+        CIB_REQUIRE(e == cudaSuccess, "attention_kv4_decode: launch failed: %s", cudaGetErrorString(e));                                             \
+        return 0;                                                                                                                                    \
+    }                                                                                                                                                \
     if (d == DV) {                                                                                                                                   \
         static SmemLimit limit;                                                                                                                      \
-        if (int rc = raise_smem_limit(limit, kv4::attention_decode_kernel<DV>, kv4::ring_bytes<DV>(), "attention_kv4_decode")) return rc;            \
-        cudaError_t e = launch_pdl(kv4::attention_decode_kernel<DV>, dim3(ctas), dim3(kv4::kDecWarps * 32), (size_t)kv4::ring_bytes<DV>(), stream,   \
-                                   use_pdl != 0, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, (const unsigned char*)cache,     \
-                                   num_pages, page_size, block_table, table_stride, query_start_loc, seq_lens, num_requests, nq, nkv, scale_log2,    \
-                                   window, unit, scratch, part_ml, error_flag);                                                                      \
+        if (int rc = raise_smem_limit(limit, kv4::attention_decode_kernel<DV, false>, kv4::ring_bytes<DV>(), "attention_kv4_decode")) return rc;     \
+        cudaError_t e = launch_pdl(kv4::attention_decode_kernel<DV, false>, dim3(ctas), dim3(kv4::kDecWarps * 32), (size_t)kv4::ring_bytes<DV>(),    \
+                                   stream, use_pdl != 0, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride,                         \
+                                   (const unsigned char*)cache, num_pages, page_size, block_table, table_stride, query_start_loc, seq_lens,         \
+                                   num_requests, nq, nkv, scale_log2, window, unit, scratch, part_ml, error_flag);                                  \
         if (e == cudaSuccess && scratch != nullptr)                                                                                                  \
             e = launch_pdl(kv4::attention_decode_merge_kernel<DV>, dim3(nq, num_requests), dim3(DV), 0, stream, use_pdl != 0, (__nv_bfloat16*)out,   \
                            out_stride, query_start_loc, seq_lens, num_requests, nq, nkv, window, unit, ctas, scratch, part_ml);                      \

@@ -123,7 +123,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "cib_kv4_read": [_P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
         "cib_attention_kv4_generic": [_P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
         "cib_attention_kv4_prompt": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P],
-        "cib_attention_kv4_decode": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _P, _P, _I, _P],
+        "cib_attention_kv4_decode": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _I, _P, _P, _I, _P],
         "cib_gemm_skinny": [_P, _I, _I, _I, _P, _I, _P, _P, _I, _P, _I, _F, _P, _P, _I, _I, _I, _I, _I, _P, ctypes.c_longlong, _P, _I, _P, _P, _P],
         "cib_gemm_tcgen05": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P, _I, _F, _P, _P, _I, _P, _P, _P],
         "cib_gemm_wstream": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _P, _I, _F, _P, _P, _I, _P, _P, _I, _P, ctypes.c_longlong, _I, _P, _P],
@@ -917,13 +917,13 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
     # request may then bring a single token.
     if (dtype == BF16 and (bound or 1 in query_lens_host) and lib.cib_attention_kv4_decode_supports(head_dim, page_size) and q_args[1] % 8 == 0
             and q_args[0] % 16 == 0):
-        ctas, unit = kv4_decode_shape(R * num_kv_heads * -(-(num_q_heads // num_kv_heads) // 8), min(max_seq_len, window + 16 if window else max_seq_len),
-                                      lib.cib_attention_kv4_decode_ctas(head_dim))
+        cluster, ctas, unit = kv4_decode_shape(R * num_kv_heads * -(-(num_q_heads // num_kv_heads) // 8),
+                                               min(max_seq_len, window + KV4_BLOCK if window else max_seq_len), lib.cib_attention_kv4_decode_ctas(head_dim))
         scratch = None
-        if min(max_seq_len, window + 16 if window else max_seq_len) > unit * KV4_BLOCK:
+        if unit:
             scratch = torch.empty(lib.cib_attention_kv4_decode_scratch_floats(head_dim, ctas), dtype=torch.float32, device=q.device)
-        rc = lib.cib_attention_kv4_decode(*q_args, *out_args, *cache_args, R, num_q_heads, num_kv_heads, head_dim, float(scale), int(window), ctas, unit,
-                                          scratch.data_ptr() if scratch is not None else None, _error_flag(q.device).data_ptr(), pdl, _stream())
+        rc = lib.cib_attention_kv4_decode(*q_args, *out_args, *cache_args, R, num_q_heads, num_kv_heads, head_dim, float(scale), int(window), cluster, ctas,
+                                          unit, scratch.data_ptr() if scratch is not None else None, _error_flag(q.device).data_ptr(), pdl, _stream())
         _check(rc, who)
         note_flagged_launch()
         _count()
@@ -950,11 +950,22 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
     _count()
 
 
+KV4_CLUSTER_MAX_KEYS = 1024
+
+
 def kv4_decode_shape(pairs: int, keys: int, slots: int) -> tuple:
-    """(CTAs, blocks of 16 keys that a CTA takes at least) of the 4-bit decode attention, for ``pairs`` (request, head block) of at most
-    ``keys`` keys on a GPU that holds ``slots`` of its CTAs: contexts of up to 512 keys are not split."""
-    unit = 32 if keys <= 512 else 8
-    return max(1, min(slots, pairs * -(-keys // (unit * KV4_BLOCK)))), unit
+    """(CTAs of a cluster, CTAs of the list, blocks of 16 keys in a unit of the list) of the 4-bit decode attention, for ``pairs`` (request, head
+    block) of at most ``keys`` keys on a GPU that holds ``slots`` of its CTAs.  A cluster (1, 2, 4 or 8 CTAs a pair, 0: none) where that
+    leaves a CTA at most ``KV4_CLUSTER_MAX_KEYS`` keys and all CTAs fit the GPU at once; with more keys a CTA, equal shares of the list
+    make up for the second kernel.  More pairs than CTAs of short contexts (up to 512 keys): whole pairs as units (0)."""
+    cluster = 8
+    while cluster > 1 and (pairs * cluster > slots or (cluster // 2) * 8 * KV4_BLOCK >= keys):       # (128 keys a CTA at least)
+        cluster //= 2
+    if pairs * cluster <= slots and keys <= cluster * KV4_CLUSTER_MAX_KEYS:
+        return cluster, 0, 0
+    if keys <= 512:
+        return 0, min(slots, pairs), 0
+    return 0, max(1, min(slots, pairs * -(-keys // (8 * KV4_BLOCK)))), 8
 
 
 # ---- matrix product ----------------------------------------------------------------------------------

@@ -572,3 +572,23 @@ def test_a_scale_that_is_not_positive():
             c = case([90, 70], [new, new], 4, 2, 128, 16, BF16, seed=3)
             c["scale"] = scale
             check(c)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 300])
+@pytest.mark.parametrize("shape", [(1, 0, 0), (2, 0, 0), (4, 0, 0), (8, 0, 0), (0, 5, 0), (0, 3, 8), (0, 64, 1), (0, 592, 8)])
+def test_every_way_to_share_the_keys_of_single_tokens(monkeypatch, d, window, shape):
+    """Clusters of every size, whole requests, and a list cut into any shares; among requests that bring several tokens or none."""
+    monkeypatch.setattr(kernels, "kv4_decode_shape", lambda *args: shape)
+    lengths, new = [700, 1, 33, 90, 410, 128, 0, 17, 259], [1, 1, 1, 40, 1, 1, 0, 1, 1]
+    c = case(lengths, new, 6, 2, d, 16, BF16, window=window, seed=d, spare_rows=1)
+    check(c)
+    c = case([513, 0, 20], [1, 1, 1], 20, 2, d, 48, BF16, window=window, seed=d)
+    check(c)
+
+
+def test_how_the_keys_of_single_tokens_are_shared():
+    assert kernels.kv4_decode_shape(8, 300, 592) == (4, 0, 0) and kernels.kv4_decode_shape(64, 4096, 592) == (8, 0, 0)
+    assert kernels.kv4_decode_shape(8, 100, 592) == (1, 0, 0) and kernels.kv4_decode_shape(128, 4096, 592) == (4, 0, 0)
+    assert kernels.kv4_decode_shape(512, 8192, 592) == (0, 592, 8) and kernels.kv4_decode_shape(32, 120001, 592) == (0, 592, 8)
+    assert kernels.kv4_decode_shape(2000, 300, 592) == (0, 592, 0)
