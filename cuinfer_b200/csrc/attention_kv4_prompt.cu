@@ -19,6 +19,10 @@
 // Which two tiles: neighbours where there are more CTAs than SMs (they see almost the same keys); else tile i and the last but i of a
 // request (`folded`), so that all CTAs of a launch that fits the GPU at once have the same work.
 //
+// Where a launch would leave SMs without work, the key tiles of a CTA are cut over several (`gridDim.z`); each then writes its rows' maximum, sum and
+// weighted values, 32-bit, to scratch memory that the caller brings, and a second kernel joins them: three portions of up to 500 tokens behind up to
+// 3 500 others (72 CTAs without) took 116 us, 62 so.
+//
 // Every mbarrier wait is bounded; on a time-out the kernel raises the error flag, stops, frees its tensor memory and returns.
 #include "kv4.cuh"
 #include "mma_utils.cuh"
@@ -62,6 +66,13 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
     return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
+// Loads that stay where they are written, a tile ahead of their use (the compiler moved plain ones down to it: 59 us for a prompt of 2 048 tokens
+// instead of 53).
+__device__ __forceinline__ void fetch(Words<4>& x, const Words<4>* p) {
+    asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.w[0]), "=r"(x.w[1]), "=r"(x.w[2]), "=r"(x.w[3]) : "l"(p));
+}
+__device__ __forceinline__ void fetch(Words<2>& x, const Words<2>* p) { asm volatile("ld.global.nc.v2.b32 {%0, %1}, [%2];" : "=r"(x.w[0]), "=r"(x.w[1]) : "l"(p)); }
+__device__ __forceinline__ void fetch(Words<1>& x, const Words<1>* p) { asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(x.w[0]) : "l"(p)); }
 // D = F32, A = B = BF16, both K-major, M = 128
 __host__ __device__ constexpr uint32_t idesc(int n) { return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t id, uint32_t acc) {
@@ -120,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* __restrict__ out, int out_stride,
                         const unsigned char* __restrict__ cache, int num_pages, int page_size, const int* __restrict__ block_table, int table_stride,
                         const int* __restrict__ query_start_loc, const int* __restrict__ seq_lens, int num_requests, int least_query, int nq, int nkv,
-                        float scale_log2, int window, int folded, int* __restrict__ error_flag) {
+                        float scale_log2, int window, int folded, float* __restrict__ part_o, float* __restrict__ part_ml, int num_tokens, int* __restrict__ error_flag) {
     constexpr int NG = D / kGroup, HG = NG / 2;
     constexpr int kBytes = block_bytes(D);
     using S = Smem<D>;
@@ -218,6 +229,12 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             const int keys = seq_len - n + last / g + 1;              // that the tile's last row sees, from the first on
             tiles[t] = has[t] && keys > k_lo ? (keys - k_lo + kN - 1) / kN : 0;
         }
+    }
+    if (gridDim.z > 1) {                        // this CTA's share of the key tiles
+        const int share = (max(tiles[0], tiles[1]) + (int)gridDim.z - 1) / (int)gridDim.z, j0 = (int)blockIdx.z * share;
+        k_lo += j0 * kN;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) tiles[t] = min(max(tiles[t] - j0, 0), share);
     }
     const int most = max(tiles[0], tiles[1]);
 
@@ -338,8 +355,8 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
                 const unsigned char* kb = cache + (size_t)max(x.id, 0) * kBytes;       // (a block that is not there: any other, its scores are replaced)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    x.c[h] = reinterpret_cast<const Words<NG>*>(kb)[(token + 8 * h) * 4 + quarter];
-                    x.w[h] = reinterpret_cast<const Words<HG>*>(kb + key_words_at(D))[token + 8 * h];
+                    fetch(x.c[h], reinterpret_cast<const Words<NG>*>(kb) + (token + 8 * h) * 4 + quarter);
+                    fetch(x.w[h], reinterpret_cast<const Words<HG>*>(kb + key_words_at(D)) + token + 8 * h);
                 }
                 return x;
             };
@@ -379,6 +396,7 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             const int octet = lane & 7, eighth = (take >> 1) * 4 + (lane >> 3), g0 = (take & 1) * HG;
             struct Codes {
                 Words<HG> c[4], w[4];
+                int id;
             };
             // lanes 4 i .. 4 i + 3: the blocks of tile 8 n + i
             int ids = lookup(lane >> 2, lane & 3), ids_next = -1;
@@ -386,15 +404,12 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
                 Codes x;
                 if ((j & 7) == 0 && j != 0) ids = ids_next;
                 if ((j & 7) == 4) ids_next = lookup((j & ~7) + 8 + (lane >> 2), lane & 3);
-                const int id = __shfl_sync(0xffffffffu, ids, (j & 7) * 4 + (octet >> 1));
-                const unsigned char* vb = cache + (size_t)max(id, 0) * kBytes;
+                x.id = __shfl_sync(0xffffffffu, ids, (j & 7) * 4 + (octet >> 1));
+                const unsigned char* vb = cache + (size_t)max(x.id, 0) * kBytes;
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
-                    x.c[p] = reinterpret_cast<const Words<HG>*>(vb + value_codes_at(D))[(((octet & 1) * 8 + eighth) * 4 + p) * 2 + (take & 1)];
-                    x.w[p] = reinterpret_cast<const Words<HG>*>(vb + value_words_at(D))[((octet & 1) * 4 + p) * 2 + (take & 1)];
-                    if (id < 0)                                     // of no page: the weights are zero
-#pragma unroll
-                        for (int k = 0; k < HG; ++k) x.w[p].w[k] = 0;
+                    fetch(x.c[p], reinterpret_cast<const Words<HG>*>(vb + value_codes_at(D)) + (((octet & 1) * 8 + eighth) * 4 + p) * 2 + (take & 1));
+                    fetch(x.w[p], reinterpret_cast<const Words<HG>*>(vb + value_words_at(D)) + ((octet & 1) * 4 + p) * 2 + (take & 1));
                 }
                 return x;
             };
@@ -404,11 +419,11 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
                 const int key0 = k_lo + j * kN;
                 Codes x = next;
                 if (j + 1 < most) next = load(j + 1);
-                if (key0 + kN > seq_len) {                          // keys behind the last one: so are theirs
+                if (key0 + kN > seq_len || __any_sync(0xffffffffu, x.id < 0)) {      // keys behind the last one, and of no page: their weights are zero
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
                         const int key = key0 + octet * 8 + 2 * p;
-                        const uint32_t keep = (key < seq_len ? 0xffffu : 0u) | (key + 1 < seq_len ? 0xffff0000u : 0u);
+                        const uint32_t keep = x.id < 0 ? 0u : (key < seq_len ? 0xffffu : 0u) | (key + 1 < seq_len ? 0xffff0000u : 0u);
 #pragma unroll
                         for (int k = 0; k < HG; ++k) x.w[p].w[k] &= keep;
                     }
@@ -559,7 +574,8 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
         unsigned char* stage = sQ + t * S::kQ;                      // (every S has read the queries)
         constexpr int kPieces = D / 8;                              // 16-byte pieces of a row
         if (*(volatile int*)&s_abort == 0 && has[t]) {
-            const float f = l == 0.f ? 0.f : __fdividef(1.f, l);
+            const bool whole = gridDim.z == 1;
+            const float f = !whole ? 1.f : l == 0.f ? 0.f : __fdividef(1.f, l);
             unsigned bad = 0;                           // groups whose sum holds a value that is not a number
             if (*(volatile int*)&s_odd && row_ok) {
                 const int* table = block_table + (size_t)r * table_stride;
@@ -583,6 +599,18 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
                     for (int e = 0; e < 32; ++e) o[e] = 0;
                 }
                 const float ff = (bad >> (c / kGroup)) & 1u ? NAN : f;
+                if (!whole) {
+                    if (row_ok) {
+                        const int tl = grow / g;
+                        const size_t at = ((size_t)blockIdx.z * num_tokens + q0 + tl) * nq + kvh * g + (grow - tl * g);
+                        if (c == 0) part_ml[at * 2] = m_used, part_ml[at * 2 + 1] = l;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            *reinterpret_cast<float4*>(part_o + at * D + c + e) = make_float4(__uint_as_float(o[e]) * ff, __uint_as_float(o[e + 1]) * ff,
+                                                                                          __uint_as_float(o[e + 2]) * ff, __uint_as_float(o[e + 3]) * ff);
+                    }
+                    continue;
+                }
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) {
                     uint4 pk;
@@ -596,7 +624,7 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             }
         }
         asm volatile("bar.sync %0, 128;" ::"r"(11 + t) : "memory");
-        if (*(volatile int*)&s_abort == 0 && has[t]) {
+        if (*(volatile int*)&s_abort == 0 && has[t] && gridDim.z == 1) {
 #pragma unroll
             for (int u = 0; u < kM * kPieces / 128; ++u) {
                 const int idx = row_local + u * 128;
@@ -615,6 +643,43 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kTmemCols) : "memory");
 }
 
+// A warp per (token, query head): joins the shares of the keys.
+template <int D>
+__global__ void __launch_bounds__(128)
+attention_prompt_merge_kernel(__nv_bfloat16* __restrict__ out, int out_stride, const int* __restrict__ query_start_loc, int num_requests, int least_query, int nq,
+                              int shares, int num_tokens, const float* __restrict__ part_o, const float* __restrict__ part_ml) {
+    const int lane = threadIdx.x & 31;
+    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int t = (int)(item / nq), head = (int)(item - (long long)t * nq);
+    if (t >= num_tokens) return;                                   // (no barrier follows)
+    int before = 0;                                                // the request of this row: the last one that starts at or before it
+    for (int r0 = 0; r0 <= num_requests; r0 += 32) {
+        const int r = r0 + lane;
+        before += __popc(__ballot_sync(0xffffffffu, r <= num_requests && query_start_loc[min(r, num_requests)] <= t));
+    }
+    griddep_wait();
+    griddep_launch();
+    const int r = before - 1;
+    if (r < 0 || r >= num_requests || query_start_loc[r + 1] - query_start_loc[r] < least_query) return;
+    constexpr int E = D / 32;
+    float M = -INFINITY, L = 0.f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    for (int z = 0; z < shares; ++z) M = fmaxf(M, part_ml[(((size_t)z * num_tokens + t) * nq + head) * 2]);
+    for (int z = 0; z < shares; ++z) {
+        const size_t at = ((size_t)z * num_tokens + t) * nq + head;
+        const float m = part_ml[at * 2];
+        const float f = m == -INFINITY ? 0.f : exp2f(m - M);
+        L += part_ml[at * 2 + 1] * f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += part_o[at * D + lane * E + e] * f;
+    }
+    const float f = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int e = 0; e < E; e += 2)
+        *reinterpret_cast<uint32_t*>(out + (size_t)t * out_stride + (size_t)head * D + lane * E + e) = pack_bf16(o[e] * f, o[e + 1] * f);
+}
+
 // The registers that a launch gives a thread: the split among the warps counts on them.
 template <typename Kernel>
 static int launch_registers(Kernel kernel) {
@@ -630,29 +695,38 @@ using namespace cib;
 extern "C" int cib_attention_kv4_prompt_supports(int d, int page_size) { return kv4::sizes_ok(d, page_size) && (d == 64 || d == 128); }
 
 // num_pairs = sum over requests of ceil(tokens_r * (nq / nkv) / 256), or more: CTAs that find none leave.  least_query: requests that bring
-// fewer tokens are left as they are.
+// fewer tokens are left as they are.  shares: how many CTAs share the keys of a pair of row tiles; scratch: shares * num_tokens * nq * (d + 2) floats where
+// there are several.
 extern "C" int cib_attention_kv4_prompt(const void* q, int q_stride, void* out, int out_stride, const void* cache, int num_pages, int page_size,
                                         const int* block_table, int table_stride, const int* query_start_loc, const int* seq_lens, int num_requests,
-                                        int num_pairs, int folded, int least_query, int nq, int nkv, int d, float scale, int window, int* error_flag,
+                                        int num_tokens, int num_pairs, int folded, int shares, int least_query, int nq, int nkv, int d, float scale, int window, float* scratch, int* error_flag,
                                         cudaStream_t stream) {
     CIB_REQUIRE(cib_attention_kv4_prompt_supports(d, page_size), "attention_kv4_prompt: head size %d (64 or 128), page size %d (a multiple of 16) are not taken", d, page_size);
     CIB_REQUIRE(num_requests >= 0 && nq > 0 && nkv > 0 && nq % nkv == 0 && num_pairs >= 0 && num_pairs <= 65535, "attention_kv4_prompt: bad sizes");
     CIB_REQUIRE(num_pages > 0 && table_stride > 0 && cache != nullptr && ((uintptr_t)cache % 16) == 0, "attention_kv4_prompt: bad cache geometry");
     CIB_REQUIRE((long long)num_pages * nkv * (page_size / kv4::kBlock) < (1ll << 31), "attention_kv4_prompt: more than 2^31 blocks");
     CIB_REQUIRE(q_stride % 8 == 0 && ((uintptr_t)q % 16) == 0 && out_stride % 8 == 0 && ((uintptr_t)out % 16) == 0, "attention_kv4_prompt: rows must be 16-byte aligned");
+    CIB_REQUIRE(shares >= 1 && shares <= 65535 && (shares == 1 || (scratch != nullptr && (uintptr_t)scratch % 16 == 0)), "attention_kv4_prompt: %d shares need scratch", shares);
+    CIB_REQUIRE((long long)num_tokens * nq < (1ll << 31), "attention_kv4_prompt: too many rows");
     CIB_REQUIRE(window >= 0 && error_flag != nullptr, "attention_kv4_prompt: window must be >= 0, error flag given");
     if (num_requests == 0 || num_pairs == 0) return 0;
     const float scale_log2 = scale * 1.4426950408889634f;
+    float* part_ml = shares > 1 ? scratch + (size_t)shares * num_tokens * nq * d : nullptr;
 #define CIB_KV4_PROMPT(DV)                                                                                                                          \
     if (d == DV) {                                                                                                                                  \
         static SmemLimit limit;                                                                                                                     \
         if (int rc = raise_smem_limit(limit, kv4p::attention_prompt_kernel<DV>, kv4p::Smem<DV>::kTotal, "attention_kv4_prompt")) return rc;         \
         static const int regs = kv4p::launch_registers(kv4p::attention_prompt_kernel<DV>);                                                          \
         CIB_REQUIRE(regs == kv4p::kLaunchRegs, "attention_kv4_prompt: built with %d registers a thread, laid out for %d", regs, kv4p::kLaunchRegs); \
-        const cudaError_t e = launch_pdl(kv4p::attention_prompt_kernel<DV>, dim3(nkv, num_pairs), dim3(kv4p::kThreads), (size_t)kv4p::Smem<DV>::kTotal, \
-                                         stream, prompt_pdl(), (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride,                  \
-                                         (const unsigned char*)cache, num_pages, page_size, block_table, table_stride, query_start_loc, seq_lens,   \
-                                         num_requests, least_query, nq, nkv, scale_log2, window, folded, error_flag);                              \
+        cudaError_t e = launch_pdl(kv4p::attention_prompt_kernel<DV>, dim3(nkv, num_pairs, shares), dim3(kv4p::kThreads),                           \
+                                   (size_t)kv4p::Smem<DV>::kTotal, stream, prompt_pdl(), (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out,    \
+                                   out_stride, (const unsigned char*)cache, num_pages, page_size, block_table, table_stride, query_start_loc,       \
+                                   seq_lens, num_requests, least_query, nq, nkv, scale_log2, window, folded, scratch, part_ml, num_tokens,          \
+                                   error_flag);                                                                                                     \
+        if (e == cudaSuccess && shares > 1)                                                                                                         \
+            e = launch_pdl(kv4p::attention_prompt_merge_kernel<DV>, dim3((unsigned)(((long long)num_tokens * nq + 3) / 4)), dim3(128), 0, stream,   \
+                           prompt_pdl(), (__nv_bfloat16*)out, out_stride, query_start_loc, num_requests, least_query, nq, shares, num_tokens,       \
+                           scratch, part_ml);                                                                                                       \
         CIB_REQUIRE(e == cudaSuccess, "attention_kv4_prompt: launch failed: %s", cudaGetErrorString(e));                                            \
         return 0;                                                                                                                                   \
     }

@@ -122,7 +122,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "cib_qk_norm_rope_kv4_write": [_P, _I, _I, _P, _I, _P, _P, _P, _P, _I, _I, _F, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P],
         "cib_kv4_read": [_P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
         "cib_attention_kv4_generic": [_P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
-        "cib_attention_kv4_prompt": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P],
+        "cib_attention_kv4_prompt": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P],
         "cib_attention_kv4_decode": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _I, _P, _P, _I, _P],
         "cib_gemm_skinny": [_P, _I, _I, _I, _P, _I, _P, _P, _I, _P, _I, _F, _P, _P, _I, _I, _I, _I, _I, _P, ctypes.c_longlong, _P, _I, _P, _P, _P],
         "cib_gemm_tcgen05": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P, _I, _F, _P, _P, _I, _P, _P, _P],
@@ -937,9 +937,14 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
             pairs = T * g // 256 + R
         else:
             pairs = sum(-(-n * g // 256) for n in query_lens_host if n >= least_query)
-        folded = window <= 0 and pairs * num_kv_heads <= 148
-        rc = lib.cib_attention_kv4_prompt(*q_args, *out_args, *cache_args, R, pairs, 1 if folded else 0, least_query, num_q_heads, num_kv_heads,
-                                         head_dim, float(scale), int(window), _error_flag(q.device).data_ptr(), _stream())
+        if not pairs:
+            return
+        shares = kv4_prompt_shares(pairs * num_kv_heads, min(max_seq_len, window + max(query_lens_host) if window else max_seq_len), T * num_q_heads * head_dim)
+        scratch = torch.empty(shares * T * num_q_heads * (head_dim + 2), dtype=torch.float32, device=q.device) if shares > 1 else None
+        folded = window <= 0 and shares == 1 and pairs * num_kv_heads <= 148
+        rc = lib.cib_attention_kv4_prompt(*q_args, *out_args, *cache_args, R, T, pairs, 1 if folded else 0, shares, least_query, num_q_heads, num_kv_heads,
+                                         head_dim, float(scale), int(window), scratch.data_ptr() if scratch is not None else None,
+                                         _error_flag(q.device).data_ptr(), _stream())
         _check(rc, who)
         note_flagged_launch()
         _count()
@@ -948,6 +953,13 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
                                        head_dim, float(scale), int(window), pdl, _stream())
     _check(rc, who)
     _count()
+
+
+def kv4_prompt_shares(ctas: int, keys: int, values: int) -> int:
+    """How many CTAs share the keys of a pair of row tiles in the 4-bit prompt attention, for ``ctas`` pairs over all key heads of at most
+    ``keys`` keys: as many as the 148 SMs take at once, with 512 keys each at least, and while the partial results (``values`` numbers a
+    share, written and read) stay below 2^24 numbers."""
+    return max(1, min(148 // max(1, ctas), keys // 512, (1 << 24) // max(1, values)))
 
 
 KV4_CLUSTER_MAX_KEYS = 1024

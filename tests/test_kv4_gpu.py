@@ -592,3 +592,27 @@ def test_how_the_keys_of_single_tokens_are_shared():
     assert kernels.kv4_decode_shape(8, 100, 592) == (1, 0, 0) and kernels.kv4_decode_shape(128, 4096, 592) == (4, 0, 0)
     assert kernels.kv4_decode_shape(512, 8192, 592) == (0, 592, 8) and kernels.kv4_decode_shape(32, 120001, 592) == (0, 592, 8)
     assert kernels.kv4_decode_shape(2000, 300, 592) == (0, 592, 0)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window", [0, 150])
+@pytest.mark.parametrize("shares", [2, 3, 9])
+def test_prompts_whose_keys_are_shared(monkeypatch, d, window, shares):
+    monkeypatch.setattr(kernels, "kv4_prompt_shares", lambda *args: shares)
+    check(case([700, 33, 1, 300, 64, 410], [130, 33, 1, 2, 64, 100], 4, 2, d, 16, BF16, window=window, seed=d + shares, spare_rows=2))
+    # rows without keys, pages that are none, and bounds in the place of lengths
+    c = case([3, 200, 90], [20, 20, 20], 6, 2, d, 16, BF16, window=window, seed=d, holes=[(1, i, -1) for i in range(13)] + [(2, 1, -1)])
+    check(c)
+    check(c, attend(c, torch.full_like(c["out"], 5.0), lens=[60 + 128, 1, 1], longest=900))
+
+
+def test_a_value_that_is_no_number_in_one_share(monkeypatch):
+    monkeypatch.setattr(kernels, "kv4_prompt_shares", lambda *args: 3)
+    test_a_later_value_that_is_no_number_does_not_reach_earlier_rows(BF16, 128, 0)
+    test_a_later_value_that_is_no_number_does_not_reach_earlier_rows(BF16, 64, 24)
+
+
+def test_how_the_keys_of_prompts_are_shared():
+    assert kernels.kv4_prompt_shares(128, 2048, 2048 * 2048) == 1 and kernels.kv4_prompt_shares(72, 4000, 1100 * 2048) == 2
+    assert kernels.kv4_prompt_shares(8, 16384, 16 * 4096) == 18 and kernels.kv4_prompt_shares(8, 700, 16 * 4096) == 1
+    assert kernels.kv4_prompt_shares(1, 120000, 4096 * 128) == 32
