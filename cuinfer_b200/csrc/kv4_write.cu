@@ -288,6 +288,7 @@ write_rows_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, const in
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = stored ? to_f32(first[p].v[e]) : 0.f, x[8 + e] = stored ? to_f32(second[p].v[e]) : 0.f;
         float error = 0.f;                                           // of the values as they are computed below, at most
+        bool rough = false;                                          // the mean square has left the range in which 32 bits hold it
         if (__any_sync(0xffffffffu, kind != 2)) {
             if (has_norm) {
                 float s0 = 0.f, s1 = 0.f;
@@ -296,7 +297,8 @@ write_rows_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, const in
                 float ss = s0 + s1;
 #pragma unroll
                 for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                const float factor = kind == 2 ? 1.f : rsqrtf(ss / (float)D + eps);
+                const float mean = ss / (float)D + eps, factor = kind == 2 ? 1.f : rsqrtf(mean);
+                rough = !(mean > 1e-30f && ss < 3e38f);
                 const float* gain = s_gain[kind == 0 ? 0 : 1] + 8 * li;
 #pragma unroll
                 for (int e = 0; e < 8; e += 4) {
@@ -322,6 +324,7 @@ write_rows_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, const in
                     for (int e = 0; e < 16; ++e) error = fmaxf(error, fabsf(x[e]));
                 }
                 error *= has_norm ? 6.7434958e-07f : 1.6858740e-07f;       // 2^-20.5, 2^-22.5
+                if (kind == 1 && rough) error = INFINITY;
             }
         }
         if (kind == 0 && stored) {

@@ -616,3 +616,25 @@ def test_how_the_keys_of_prompts_are_shared():
     assert kernels.kv4_prompt_shares(128, 2048, 2048 * 2048) == 1 and kernels.kv4_prompt_shares(72, 4000, 1100 * 2048) == 2
     assert kernels.kv4_prompt_shares(8, 16384, 16 * 4096) == 18 and kernels.kv4_prompt_shares(8, 700, 16 * 4096) == 1
     assert kernels.kv4_prompt_shares(1, 120000, 4096 * 128) == 32
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T", [3, 1200])
+@pytest.mark.parametrize("eps", [1e-6, 1e-36])
+def test_keys_whose_squares_leave_the_range_of_32_bits(dtype, T, eps):
+    """A row of 2^70 or 2^-70 times the others': its squares are infinite, or nothing, in 32 bits; its normed keys are like any others."""
+    nq, nkv, d, page = 4, 2, 128, 16
+    width = (nq + 2 * nkv) * d
+    qkv = rand(T, width, seed=T, dtype=dtype)
+    qkv[0, nq * d:(nq + nkv) * d] *= 2.0 ** 70
+    qkv[1, nq * d:(nq + nkv) * d] *= 2.0 ** -70
+    qkv[2, nq * d:(nq + nkv) * d] = 0.0
+    gains = [(1 + rand(d, seed=s, scale=0.3)).to(dtype).to(DEV) for s in (1, 2)]
+    table, positions = rope_table(600, d), torch.arange(T, dtype=torch.int32) % 600
+    pages = (T + page - 1) // page
+    cache = torch.zeros(kernels.kv4_cache_shape(pages, nkv, page, d), dtype=torch.uint8, device=DEV)
+    kernels.qk_norm_rope_kv4_write(qkv.to(DEV), positions.to(DEV), ints(list(range(T))), *gains, eps, table, d, cache, nq, nkv, d)
+    _, k, v = plain_rows(qkv, positions, *gains, eps, table, d, nq, nkv, d)
+    at = torch.arange(T)
+    for rows, hold in zip((k, v), P4.unpack(cache, d)):
+        assert torch.equal(hold[at // page, :, at % page], torch.from_numpy(P4.held(rows.numpy().astype(np.float32))))
