@@ -20,7 +20,7 @@ constexpr int kMaxWarps = 8;
 template <typename T>
 __global__ void __launch_bounds__(kMaxWarps * 32)
 attention_generic_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out, int out_stride, unsigned char* __restrict__ cache, int num_pages,
-                         int page_size, const int* __restrict__ block_table, int table_stride, const int* __restrict__ query_start_loc,
+                         int page_size, const int* __restrict__ block_table, int table_stride, int table_cols, const int* __restrict__ query_start_loc,
                          const int* __restrict__ seq_lens, int num_requests, int least_query, int nq, int nkv, int d, float scale, int window) {
     extern __shared__ float smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
@@ -60,7 +60,7 @@ attention_generic_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ 
     for (int c = lo + warp * 32; c <= pos; c += warps * 32) {
         const int j = c + lane;
         const unsigned char* block = nullptr;
-        if (j <= pos && j / page_size < table_stride) {
+        if (j <= pos && j / page_size < table_cols) {
             const int page = table[j / page_size];
             if (page >= 0 && page < num_pages) block = block_of(cache, page * page_size + j % page_size, num_pages, page_size, nkv, kvh, d);
         }
@@ -157,13 +157,13 @@ using namespace cib;
 // query_start_loc holds num_requests + 1 boundaries of the num_tokens rows.  longest: no request has more keys (it shapes the launch only).
 // least_query: rows of requests that bring fewer tokens are left as they are.
 extern "C" int cib_attention_kv4_generic(const void* q, int dtype, int q_stride, void* out, int out_stride, const void* cache, int num_pages, int page_size,
-                                         const int* block_table, int table_stride, const int* query_start_loc, const int* seq_lens, int num_tokens,
+                                         const int* block_table, int table_stride, int table_cols, const int* query_start_loc, const int* seq_lens, int num_tokens,
                                          int num_requests, int longest, int least_query, int nq, int nkv, int d, float scale, int window, int use_pdl,
                                          cudaStream_t stream) {
     CIB_REQUIRE(num_tokens >= 0 && nq > 0 && nkv > 0 && nq % nkv == 0, "attention_kv4: bad sizes T=%d nq=%d nkv=%d", num_tokens, nq, nkv);
     CIB_REQUIRE(kv4::sizes_ok(d, page_size), "attention_kv4: head size %d must be a multiple of 32 up to 256, page size %d a multiple of 16", d, page_size);
     CIB_REQUIRE(num_requests > 0 || num_tokens == 0, "attention_kv4: tokens without requests");
-    CIB_REQUIRE(num_pages > 0 && table_stride > 0 && cache != nullptr && ((uintptr_t)cache % 16) == 0, "attention_kv4: bad cache geometry");
+    CIB_REQUIRE(num_pages > 0 && table_stride > 0 && table_cols > 0 && cache != nullptr && ((uintptr_t)cache % 16) == 0, "attention_kv4: bad cache geometry");
     CIB_REQUIRE((long long)num_pages * page_size < (1ll << 31), "attention_kv4: %d pages of %d slots do not fit 32-bit slot numbers", num_pages, page_size);
     CIB_REQUIRE(q_stride >= nq * d && out_stride >= nq * d, "attention_kv4: row strides %d and %d are too small", q_stride, out_stride);
     CIB_REQUIRE(window >= 0, "attention_kv4: window must be >= 0 (0 = all keys)");
@@ -179,11 +179,11 @@ extern "C" int cib_attention_kv4_generic(const void* q, int dtype, int q_stride,
     cudaError_t e;
     if (dtype == kF32)
         e = launch_pdl(kv4::attention_generic_kernel<float>, grid, dim3(warps * 32), smem, stream, use_pdl != 0, (const float*)q, q_stride, (float*)out, out_stride,
-                       (unsigned char*)cache, num_pages, page_size, block_table, table_stride, query_start_loc, seq_lens, num_requests, least_query, nq, nkv, d,
+                       (unsigned char*)cache, num_pages, page_size, block_table, table_stride, table_cols, query_start_loc, seq_lens, num_requests, least_query, nq, nkv, d,
                        scale, window);
     else
         e = launch_pdl(kv4::attention_generic_kernel<__nv_bfloat16>, grid, dim3(warps * 32), smem, stream, use_pdl != 0, (const __nv_bfloat16*)q, q_stride,
-                       (__nv_bfloat16*)out, out_stride, (unsigned char*)cache, num_pages, page_size, block_table, table_stride, query_start_loc, seq_lens,
+                       (__nv_bfloat16*)out, out_stride, (unsigned char*)cache, num_pages, page_size, block_table, table_stride, table_cols, query_start_loc, seq_lens,
                        num_requests, least_query, nq, nkv, d, scale, window);
     CIB_REQUIRE(e == cudaSuccess, "attention_kv4: launch failed: %s", cudaGetErrorString(e));
     return 0;

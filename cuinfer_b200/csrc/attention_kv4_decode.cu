@@ -143,7 +143,7 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 template <int D, bool CLUSTER>
 __global__ void __launch_bounds__(kDecWarps * 32, D > 128 ? 2 : 4)
 attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* __restrict__ out, int out_stride,
-                        const unsigned char* __restrict__ cache, int num_pages, int page_size, const int* __restrict__ block_table, int table_stride,
+                        const unsigned char* __restrict__ cache, int num_pages, int page_size, const int* __restrict__ block_table, int table_stride, int table_cols,
                         const int* __restrict__ query_start_loc, const int* __restrict__ seq_lens, int num_requests, int nq, int nkv, float scale_log2, int window,
                         int unit, float* __restrict__ part_o, float* __restrict__ part_ml, int* __restrict__ error_flag) {
     constexpr int NG = D / kGroup;
@@ -151,7 +151,7 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint64_t s_full[kDecWarps * kDecStages];
     __shared__ Place s_place;
-    __shared__ int s_failed;         // a wait ran out: no further one is begun
+    __shared__ int s_failed;         // a wait ran out: no further piece of the list is begun
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, row = lane >> 2;
     const int g = nq / nkv, blocks_per_kv = (g + kDecHeads - 1) / kDecHeads, head_blocks = nkv * blocks_per_kv;
 
@@ -222,7 +222,7 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
         const int b = begin + 2 * (i * kDecWarps + warp) + (lane & 1);
         if (i >= count || b >= end) return -1;
         const int index = b / per_page;
-        if (index >= table_stride) return -1;
+        if (index >= table_cols) return -1;
         const int page = table[index];
         return page >= 0 && page < num_pages ? (page * nkv + kvh) * per_page + (b - index * per_page) : -1;
     };
@@ -425,8 +425,8 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
     };
     // stage i has landed (false: the wait ran out); the stage that pair i - 2 was read from is refilled
     auto arrive = [&](int i) {
-        bool landed = mbar_try_wait(&full[st], parity);
-        if (!landed) landed = *(volatile int*)&s_failed == 0 && mbar_wait(&full[st], parity);
+        // (every warp waits for its own copies, of which one pair of blocks is on its way here, also where another warp's wait has run out)
+        const bool landed = mbar_try_wait(&full[st], parity) || mbar_wait(&full[st], parity);
         if (!__all_sync(0xffffffffu, landed)) {
             if (lane == 0) atomicExch(error_flag, 41), *(volatile int*)&s_failed = 1;
             return false;
@@ -528,7 +528,7 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
         }
         cluster.sync();                                           // (a CTA's shared memory has been read before it leaves)
     }
-    __syncthreads();     // (the rings are filled again)
+    if (__syncthreads_or(*(volatile int*)&s_failed)) break;       // (the rings are filled again)
     }
 }
 
@@ -616,14 +616,14 @@ extern "C" long long cib_attention_kv4_decode_scratch_floats(int d, int ctas) { 
 // of 16 keys that a CTA has at least.  scratch: cib_attention_kv4_decode_scratch_floats, or none where no request has more than `unit`
 // blocks (no request is split then, whatever its length).
 extern "C" int cib_attention_kv4_decode(const void* q, int q_stride, void* out, int out_stride, const void* cache, int num_pages, int page_size,
-                                        const int* block_table, int table_stride, const int* query_start_loc, const int* seq_lens, int num_requests, int nq,
+                                        const int* block_table, int table_stride, int table_cols, const int* query_start_loc, const int* seq_lens, int num_requests, int nq,
                                         int nkv, int d, float scale, int window, int cluster, int ctas, int unit, float* scratch, int* error_flag, int use_pdl,
                                         cudaStream_t stream) {
     CIB_REQUIRE(cib_attention_kv4_decode_supports(d, page_size), "attention_kv4_decode: head size %d (64, 128 or 256), page size %d (a multiple of 16) are not taken", d, page_size);
     CIB_REQUIRE(num_requests >= 0 && num_requests <= 65535 && nq > 0 && nkv > 0 && nq % nkv == 0, "attention_kv4_decode: bad sizes R=%d nq=%d nkv=%d", num_requests, nq, nkv);
     CIB_REQUIRE(cluster == 0 || cluster == 1 || cluster == 2 || cluster == 4 || cluster == kv4::kDecCluster, "attention_kv4_decode: clusters of 1, 2, 4 or 8, not %d", cluster);
     CIB_REQUIRE(cluster > 0 || (ctas >= 1 && (scratch == nullptr || (unit >= 1 && unit <= 1 << 20))), "attention_kv4_decode: bad launch shape %d, %d", ctas, unit);
-    CIB_REQUIRE(num_pages > 0 && table_stride > 0 && cache != nullptr && ((uintptr_t)cache % 16) == 0, "attention_kv4_decode: bad cache geometry");
+    CIB_REQUIRE(num_pages > 0 && table_stride > 0 && table_cols > 0 && cache != nullptr && ((uintptr_t)cache % 16) == 0, "attention_kv4_decode: bad cache geometry");
     CIB_REQUIRE((long long)num_pages * nkv * (page_size / kv4::kBlock) < (1ll << 31), "attention_kv4_decode: more than 2^31 blocks");
     CIB_REQUIRE(q_stride % 8 == 0 && ((uintptr_t)q % 16) == 0, "attention_kv4_decode: query rows must be 16-byte aligned");
     CIB_REQUIRE(window >= 0 && error_flag != nullptr, "attention_kv4_decode: window must be >= 0, error flag given");
@@ -640,7 +640,7 @@ extern "C" int cib_attention_kv4_decode(const void* q, int q_stride, void* out, 
         const cudaError_t e = launch_pdl_cluster(kv4::attention_decode_kernel<DV, true>, dim3(cluster, (unsigned)pairs), dim3(kv4::kDecWarps * 32),  \
                                                  (size_t)kv4::ring_bytes<DV>(), stream, use_pdl != 0, cluster, (const __nv_bfloat16*)q, q_stride,    \
                                                  (__nv_bfloat16*)out, out_stride, (const unsigned char*)cache, num_pages, page_size, block_table,    \
-                                                 table_stride, query_start_loc, seq_lens, num_requests, nq, nkv, scale_log2, window, 1,              \
+                                                 table_stride, table_cols, query_start_loc, seq_lens, num_requests, nq, nkv, scale_log2, window, 1,  \
                                                  nullptr, nullptr, error_flag);                                                                      \
         CIB_REQUIRE(e == cudaSuccess, "attention_kv4_decode: launch failed: %s", cudaGetErrorString(e));                                             \
         return 0;                                                                                                                                    \
@@ -650,8 +650,8 @@ extern "C" int cib_attention_kv4_decode(const void* q, int q_stride, void* out, 
         if (int rc = raise_smem_limit(limit, kv4::attention_decode_kernel<DV, false>, kv4::ring_bytes<DV>(), "attention_kv4_decode")) return rc;     \
         cudaError_t e = launch_pdl(kv4::attention_decode_kernel<DV, false>, dim3(ctas), dim3(kv4::kDecWarps * 32), (size_t)kv4::ring_bytes<DV>(),    \
                                    stream, use_pdl != 0, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride,                         \
-                                   (const unsigned char*)cache, num_pages, page_size, block_table, table_stride, query_start_loc, seq_lens,         \
-                                   num_requests, nq, nkv, scale_log2, window, unit, scratch, part_ml, error_flag);                                  \
+                                   (const unsigned char*)cache, num_pages, page_size, block_table, table_stride, table_cols, query_start_loc,       \
+                                   seq_lens, num_requests, nq, nkv, scale_log2, window, unit, scratch, part_ml, error_flag);                        \
         if (e == cudaSuccess && scratch != nullptr)                                                                                                  \
             e = launch_pdl(kv4::attention_decode_merge_kernel<DV>, dim3(nq, num_requests), dim3(DV), 0, stream, use_pdl != 0, (__nv_bfloat16*)out,   \
                            out_stride, query_start_loc, seq_lens, num_requests, nq, nkv, window, unit, ctas, scratch, part_ml);                      \

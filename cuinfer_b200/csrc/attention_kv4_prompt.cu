@@ -129,7 +129,7 @@ struct Smem {
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* __restrict__ out, int out_stride,
-                        const unsigned char* __restrict__ cache, int num_pages, int page_size, const int* __restrict__ block_table, int table_stride,
+                        const unsigned char* __restrict__ cache, int num_pages, int page_size, const int* __restrict__ block_table, int table_stride, int table_cols,
                         const int* __restrict__ query_start_loc, const int* __restrict__ seq_lens, int num_requests, int least_query, int nq, int nkv,
                         float scale_log2, int window, int folded, float* __restrict__ part_o, float* __restrict__ part_ml, int num_tokens, int* __restrict__ error_flag) {
     constexpr int NG = D / kGroup, HG = NG / 2;
@@ -328,7 +328,7 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
         // the number of block `block` of key tile j, or -1 (no such tile, behind the last key, or not named by the table)
         auto lookup = [&](int j, int block) {
             const int b = (k_lo + j * kN) / kBlock + block, index = b / per_page;
-            if (j >= most || b * kBlock >= seq_len || index >= table_stride) return -1;
+            if (j >= most || b * kBlock >= seq_len || index >= table_cols) return -1;
             const int page = __ldg(table + index);
             return page >= 0 && page < num_pages ? (page * nkv + kvh) * per_page + (b - index * per_page) : -1;
         };
@@ -579,7 +579,7 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             unsigned bad = 0;                           // groups whose sum holds a value that is not a number
             if (*(volatile int*)&s_odd && row_ok) {
                 const int* table = block_table + (size_t)r * table_stride;
-                for (int key = window > 0 ? max(0, pos - window + 1) : 0; key <= pos && key / page_size < table_stride; ++key) {
+                for (int key = window > 0 ? max(0, pos - window + 1) : 0; key <= pos && key / page_size < table_cols; ++key) {
                     const int page = table[key / page_size];
                     if (page < 0 || page >= num_pages) continue;
                     const unsigned char* block = cache + ((size_t)(page * nkv + kvh) * (page_size / kBlock) + key % page_size / kBlock) * kBytes;
@@ -698,12 +698,12 @@ extern "C" int cib_attention_kv4_prompt_supports(int d, int page_size) { return 
 // fewer tokens are left as they are.  shares: how many CTAs share the keys of a pair of row tiles; scratch: shares * num_tokens * nq * (d + 2) floats where
 // there are several.
 extern "C" int cib_attention_kv4_prompt(const void* q, int q_stride, void* out, int out_stride, const void* cache, int num_pages, int page_size,
-                                        const int* block_table, int table_stride, const int* query_start_loc, const int* seq_lens, int num_requests,
+                                        const int* block_table, int table_stride, int table_cols, const int* query_start_loc, const int* seq_lens, int num_requests,
                                         int num_tokens, int num_pairs, int folded, int shares, int least_query, int nq, int nkv, int d, float scale, int window, float* scratch, int* error_flag,
                                         cudaStream_t stream) {
     CIB_REQUIRE(cib_attention_kv4_prompt_supports(d, page_size), "attention_kv4_prompt: head size %d (64 or 128), page size %d (a multiple of 16) are not taken", d, page_size);
     CIB_REQUIRE(num_requests >= 0 && nq > 0 && nkv > 0 && nq % nkv == 0 && num_pairs >= 0 && num_pairs <= 65535, "attention_kv4_prompt: bad sizes");
-    CIB_REQUIRE(num_pages > 0 && table_stride > 0 && cache != nullptr && ((uintptr_t)cache % 16) == 0, "attention_kv4_prompt: bad cache geometry");
+    CIB_REQUIRE(num_pages > 0 && table_stride > 0 && table_cols > 0 && cache != nullptr && ((uintptr_t)cache % 16) == 0, "attention_kv4_prompt: bad cache geometry");
     CIB_REQUIRE((long long)num_pages * nkv * (page_size / kv4::kBlock) < (1ll << 31), "attention_kv4_prompt: more than 2^31 blocks");
     CIB_REQUIRE(q_stride % 8 == 0 && ((uintptr_t)q % 16) == 0 && out_stride % 8 == 0 && ((uintptr_t)out % 16) == 0, "attention_kv4_prompt: rows must be 16-byte aligned");
     CIB_REQUIRE(shares >= 1 && shares <= 65535 && (shares == 1 || (scratch != nullptr && (uintptr_t)scratch % 16 == 0)), "attention_kv4_prompt: %d shares need scratch", shares);
@@ -720,7 +720,7 @@ extern "C" int cib_attention_kv4_prompt(const void* q, int q_stride, void* out, 
         CIB_REQUIRE(regs == kv4p::kLaunchRegs, "attention_kv4_prompt: built with %d registers a thread, laid out for %d", regs, kv4p::kLaunchRegs); \
         cudaError_t e = launch_pdl(kv4p::attention_prompt_kernel<DV>, dim3(nkv, num_pairs, shares), dim3(kv4p::kThreads),                           \
                                    (size_t)kv4p::Smem<DV>::kTotal, stream, prompt_pdl(), (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out,    \
-                                   out_stride, (const unsigned char*)cache, num_pages, page_size, block_table, table_stride, query_start_loc,       \
+                                   out_stride, (const unsigned char*)cache, num_pages, page_size, block_table, table_stride, table_cols, query_start_loc, \
                                    seq_lens, num_requests, least_query, nq, nkv, scale_log2, window, folded, scratch, part_ml, num_tokens,          \
                                    error_flag);                                                                                                     \
         if (e == cudaSuccess && shares > 1)                                                                                                         \

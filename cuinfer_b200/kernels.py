@@ -121,9 +121,9 @@ def _declare(lib: ctypes.CDLL) -> None:
         "cib_attention_tcgen05": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P],
         "cib_qk_norm_rope_kv4_write": [_P, _I, _I, _P, _I, _P, _P, _P, _P, _I, _I, _F, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P],
         "cib_kv4_read": [_P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
-        "cib_attention_kv4_generic": [_P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
-        "cib_attention_kv4_prompt": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P],
-        "cib_attention_kv4_decode": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _I, _P, _P, _I, _P],
+        "cib_attention_kv4_generic": [_P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
+        "cib_attention_kv4_prompt": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P],
+        "cib_attention_kv4_decode": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _I, _P, _P, _I, _P],
         "cib_gemm_skinny": [_P, _I, _I, _I, _P, _I, _P, _P, _I, _P, _I, _F, _P, _P, _I, _I, _I, _I, _I, _P, ctypes.c_longlong, _P, _I, _P, _P, _P],
         "cib_gemm_tcgen05": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P, _I, _F, _P, _P, _I, _P, _P, _P],
         "cib_gemm_wstream": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _P, _I, _F, _P, _P, _I, _P, _P, _I, _P, ctypes.c_longlong, _I, _P, _P],
@@ -880,14 +880,15 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
                         window: int = 0, *, max_seq_len: int) -> None:
     """Causal attention of the packed query rows ``q[:, :nq*d]`` over a paged cache held in 4 bits (``kv4_cache_shape``); out[T, nq*d].
     Request r brings the rows ``query_start_loc[r]`` to ``query_start_loc[r + 1]``, the last tokens of its ``seq_lens[r]``; its pages
-    are row r of ``block_table`` (a page that is none, -1: its keys are left out).  ``window`` > 0: a query sees the last so many
+    are row r of ``block_table`` (a page that is none, -1, or behind the row's end: its keys are left out).  ``window`` > 0: a query sees the last so many
     keys.  Rows that see no key are zero; rows behind the last request are left as they are.  ``query_lens_host``: how many rows
     each request brings (host ints, or an upper bound as ``StepContext.query_lens_for_launch`` gives); ``max_seq_len``: no request
-    has more keys.  Both shape the launch only.  float32 or bfloat16."""
+    has more keys.  Both shape the launch only.  ``out`` shares no memory with ``q``.  float32 or bfloat16; in bfloat16 queries and
+    what the cache holds are below 2^120 in magnitude (steps are scaled by powers of two on the way)."""
     who = "paged_attention_kv4"
     T = q.shape[0]
     page_size = _kv4_cache(cache, num_kv_heads, head_dim, who)
-    if num_q_heads <= 0 or num_q_heads % num_kv_heads:
+    if num_q_heads <= 0 or num_kv_heads <= 0 or num_q_heads % num_kv_heads:
         raise KernelError(f"{who}: {num_q_heads} query heads do not share {num_kv_heads} key heads")
     width = num_q_heads * head_dim
     if q.dim() != 2 or q.stride(1) != 1 or q.shape[1] < width or out.shape != (T, width) or out.stride(1) != 1 or out.dtype != q.dtype:
@@ -897,15 +898,15 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
         raise KernelError(f"{who}: query_start_loc must be [R + 1], block_table [R, pages] and query_lens_host name R requests for the R = {R} of seq_lens")
     if block_table.stride(1) != 1 and block_table.shape[1] > 1:
         raise KernelError(f"{who}: block_table rows must be dense")
-    if window < 0 or max_seq_len < 0:
-        raise KernelError(f"{who}: window and max_seq_len must not be negative")
+    if not (0 <= window < 1 << 31 and 0 <= max_seq_len < 1 << 31):
+        raise KernelError(f"{who}: window and max_seq_len must not be negative, nor 2^31 or more")
     if block_table.dtype is not torch.int32:
         raise KernelError(f"{who}: block_table must be torch.int32, got {block_table.dtype}")
     _same_device(who, q, out, cache, block_table, query_start_loc, seq_lens)
     if T == 0 or R == 0:
         return
     lib = library()
-    cache_args = (_dense(cache, "cache"), cache.shape[0], page_size, block_table.data_ptr(), _row_stride(block_table),
+    cache_args = (_dense(cache, "cache"), cache.shape[0], page_size, block_table.data_ptr(), _row_stride(block_table), block_table.shape[1],
                   _dense(query_start_loc, "query_start_loc", torch.int32), _dense(seq_lens, "seq_lens", torch.int32))
     q_args = (q.data_ptr(), _row_stride(q))
     out_args = (out.data_ptr(), _row_stride(out))

@@ -151,3 +151,13 @@ def test_attention_refuses(change, match):
 def test_tensors_that_are_not_on_the_device_are_refused():
     with pytest.raises(kernels.KernelError, match="CUDA"):
         kernels.qk_norm_rope_kv4_write(**_write_args())
+
+
+@pytest.mark.parametrize("change, match", [
+    (dict(window=1 << 31), "window"),
+    (dict(max_seq_len=1 << 32), "max_seq_len"),
+    (dict(num_q_heads=0), "do not share"),
+    (dict(num_kv_heads=0, cache=torch.zeros(2, 0, 1, 18 * 64, dtype=torch.uint8)), "do not share"),
+])
+def test_attention_refuses_sizes_out_of_range(change, match):
+    test_attention_refuses(change, match)

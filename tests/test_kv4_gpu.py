@@ -638,3 +638,18 @@ def test_keys_whose_squares_leave_the_range_of_32_bits(dtype, T, eps):
     at = torch.arange(T)
     for rows, hold in zip((k, v), P4.unpack(cache, d)):
         assert torch.equal(hold[at // page, :, at % page], torch.from_numpy(P4.held(rows.numpy().astype(np.float32))))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [128, 96])
+@pytest.mark.parametrize("new", [1, 20])
+def test_a_table_that_is_a_part_of_a_wider_one(dtype, d, new):
+    """Keys behind the row's end have no page, whatever the memory behind the row holds."""
+    c = case([70, 200, 50], [new] * 3, 4, 2, d, 16, dtype, seed=d + new)
+    wide = ints([row[:6] + list(range(1, 9)) for row in c["table"]])
+    c["table"] = [row[:6] for row in c["table"]]
+    attend(c, table=wide[:, :6])
+    check(c, c["out"])
+    c["table"] = [row[2:6] for row in c["table"]]
+    attend(c, table=wide[:, 2:6])
+    check(c, c["out"])
