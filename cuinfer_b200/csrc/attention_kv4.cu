@@ -1,30 +1,35 @@
-// Paged causal attention over the cache that is held in 4 bits (kv4.cuh), the all-sizes kernel: any head size that is a
-// multiple of 32 up to 256, any head counts, 32-bit or bfloat16 queries, an optional window.
+// Paged causal attention of single tokens over the cache that is held in 4 bits (kv4.cuh), the all-sizes kernel: any head size that is a
+// multiple of 32 up to 256, any head counts, 32-bit or bfloat16 queries, an optional window.  (It takes several tokens of a request too, a token at a
+// time; attention_kv4_rows.cu shares the keys among them.)
 //
 //   out = softmax(scale * q K^T over the keys position - window < j <= position) V
 //
 // The queries of a request are the last n positions of its sequence.  A CTA takes one token and up to four query heads of one kv
 // head (a key is taken apart once for all four); its warps share the keys in chunks of 32, a key to a lane for the scores, a value
-// column to a lane for the weighted sum, and merge their running maxima and sums in shared memory.  32-bit throughout,
+// column to a lane for the weighted sum, and merge their running maxima and sums in shared memory.  Where that leaves SMs without work, a
+// cluster of up to eight CTAs shares the keys and joins its parts through distributed shared memory.  32-bit throughout,
 // the exact exponential; nothing is rounded before the end.  Keys whose page the block table does not name are left out; a row
 // without keys is zero; rows that belong to no request are left as they are.
 #include "kv4.cuh"
 #include "mma_utils.cuh"
+
+#include <cooperative_groups.h>
 
 namespace cib {
 namespace kv4 {
 
 constexpr int kHeads = 4;
 constexpr int kMaxWarps = 8;
+constexpr int kMaxCluster = 8;
 
 template <typename T>
 __global__ void __launch_bounds__(kMaxWarps * 32)
 attention_generic_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out, int out_stride, unsigned char* __restrict__ cache, int num_pages,
                          int page_size, const int* __restrict__ block_table, int table_stride, int table_cols, const int* __restrict__ query_start_loc,
-                         const int* __restrict__ seq_lens, int num_requests, int least_query, int nq, int nkv, int d, float scale, int window) {
+                         const int* __restrict__ seq_lens, int num_requests, int least_query, int nq, int nkv, int d, float scale, int window, int cluster) {
     extern __shared__ float smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    const int t = blockIdx.x, kvh = blockIdx.y;
+    const int t = blockIdx.x / cluster, rank = blockIdx.x - t * cluster, kvh = blockIdx.y;
     const int g = nq / nkv;
     const int head0 = kvh * g + blockIdx.z * kHeads;
     const int nh = min(kHeads, (kvh + 1) * g - head0);
@@ -57,7 +62,7 @@ attention_generic_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ 
 #pragma unroll
         for (int k = 0; k < kMaxHeadDim / kGroup; ++k) acc[h][k] = 0.f;
     }
-    for (int c = lo + warp * 32; c <= pos; c += warps * 32) {
+    for (int c = lo + (rank * warps + warp) * 32; c <= pos; c += cluster * warps * 32) {
         const int j = c + lane;
         const unsigned char* block = nullptr;
         if (j <= pos && j / page_size < table_cols) {
@@ -125,6 +130,7 @@ attention_generic_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ 
     }
     // merge: [warp][head][d + 2]
     float* part = smem + kHeads * d;
+    float* share = part + (size_t)warps * kHeads * (d + 2);      // of a cluster's CTA: [head][d + 2]
 #pragma unroll
     for (int h = 0; h < kHeads; ++h) {
         float* mine = part + (size_t)(warp * kHeads + h) * (d + 2);
@@ -144,9 +150,31 @@ attention_generic_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ 
             sum += from[d + 1] * f;
             o += from[x] * f;
         }
+        if (cluster > 1) {
+            share[h * (d + 2) + x] = o;
+            if (x == 0) share[h * (d + 2) + d] = top, share[h * (d + 2) + d + 1] = sum;
+            continue;
+        }
         // (a sum that is not a number stays one: only a row without keys is zero)
         out[(size_t)t * out_stride + (size_t)head0 * d + i] = from_f32<T>(sum == 0.f ? 0.f : o / sum);
     }
+    if (cluster == 1) return;
+    namespace cg = cooperative_groups;
+    cg::cluster_group group = cg::this_cluster();
+    group.sync();                                          // every CTA's part is in its shared memory
+    for (int i = rank * blockDim.x + threadIdx.x; i < nh * d; i += cluster * blockDim.x) {
+        const int h = i / d, x = i - h * d;
+        float top = -INFINITY, sum = 0.f, o = 0.f;
+        for (int c = 0; c < cluster; ++c) top = fmaxf(top, group.map_shared_rank(share, c)[h * (d + 2) + d]);
+        for (int c = 0; c < cluster; ++c) {
+            const float* from = group.map_shared_rank(share, c) + h * (d + 2);
+            const float f = from[d] == -INFINITY ? 0.f : expf(from[d] - top);
+            sum += from[d + 1] * f;
+            o += from[x] * f;
+        }
+        out[(size_t)t * out_stride + (size_t)head0 * d + i] = from_f32<T>(sum == 0.f ? 0.f : o / sum);
+    }
+    group.sync();                                          // (a CTA's shared memory has been read before it leaves)
 }
 
 }  // namespace kv4
@@ -174,17 +202,22 @@ extern "C" int cib_attention_kv4_generic(const void* q, int dtype, int q_stride,
     // a warp for every two chunks of 32 keys, so that a short context's merge stays small
     const int keys = window > 0 && window < longest ? window : longest;
     const int warps = keys <= 64 ? 1 : keys <= 128 ? 2 : keys <= 512 ? 4 : kv4::kMaxWarps;
-    const size_t smem = (size_t)(kv4::kHeads * d + warps * kv4::kHeads * (d + 2)) * sizeof(float);
-    const dim3 grid(num_tokens, nkv, (g + kv4::kHeads - 1) / kv4::kHeads);
+    // (a CTA's warps have 256 keys on their way; up to four CTAs an SM)
+    const long long ctas = (long long)num_tokens * nkv * ((g + kv4::kHeads - 1) / kv4::kHeads);
+    int cluster = 1;
+    while (cluster < kv4::kMaxCluster && ctas * cluster * 2 <= 148 * 4 && keys > cluster * 256) cluster *= 2;
+    const size_t smem = (size_t)(kv4::kHeads * d + (warps + (cluster > 1 ? 1 : 0)) * kv4::kHeads * (d + 2)) * sizeof(float);
+    CIB_REQUIRE((long long)num_tokens * cluster < (1ll << 31), "attention_kv4: too many rows");
+    const dim3 grid(num_tokens * cluster, nkv, (g + kv4::kHeads - 1) / kv4::kHeads);
     cudaError_t e;
     if (dtype == kF32)
-        e = launch_pdl(kv4::attention_generic_kernel<float>, grid, dim3(warps * 32), smem, stream, use_pdl != 0, (const float*)q, q_stride, (float*)out, out_stride,
+        e = launch_pdl_cluster(kv4::attention_generic_kernel<float>, grid, dim3(warps * 32), smem, stream, use_pdl != 0, cluster, (const float*)q, q_stride, (float*)out, out_stride,
                        (unsigned char*)cache, num_pages, page_size, block_table, table_stride, table_cols, query_start_loc, seq_lens, num_requests, least_query, nq, nkv, d,
-                       scale, window);
+                       scale, window, cluster);
     else
-        e = launch_pdl(kv4::attention_generic_kernel<__nv_bfloat16>, grid, dim3(warps * 32), smem, stream, use_pdl != 0, (const __nv_bfloat16*)q, q_stride,
+        e = launch_pdl_cluster(kv4::attention_generic_kernel<__nv_bfloat16>, grid, dim3(warps * 32), smem, stream, use_pdl != 0, cluster, (const __nv_bfloat16*)q, q_stride,
                        (__nv_bfloat16*)out, out_stride, (unsigned char*)cache, num_pages, page_size, block_table, table_stride, table_cols, query_start_loc, seq_lens,
-                       num_requests, least_query, nq, nkv, d, scale, window);
+                       num_requests, least_query, nq, nkv, d, scale, window, cluster);
     CIB_REQUIRE(e == cudaSuccess, "attention_kv4: launch failed: %s", cudaGetErrorString(e));
     return 0;
 }

@@ -122,6 +122,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "cib_qk_norm_rope_kv4_write": [_P, _I, _I, _P, _I, _P, _P, _P, _P, _I, _I, _F, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P],
         "cib_kv4_read": [_P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
         "cib_attention_kv4_generic": [_P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
+        "cib_attention_kv4_rows": [_P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
         "cib_attention_kv4_prompt": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P],
         "cib_attention_kv4_decode": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _I, _P, _P, _I, _P],
         "cib_gemm_skinny": [_P, _I, _I, _I, _P, _I, _P, _P, _I, _P, _I, _F, _P, _P, _I, _I, _I, _I, _I, _P, ctypes.c_longlong, _P, _I, _P, _P, _P],
@@ -156,6 +157,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.cib_paged_attention_decode_supports.restype = _I
     lib.cib_attention_kv4_prompt_supports.argtypes = [_I, _I]
     lib.cib_attention_kv4_prompt_supports.restype = _I
+    lib.cib_attention_kv4_rows_ctas.argtypes = [_I]
+    lib.cib_attention_kv4_rows_ctas.restype = _I
     lib.cib_attention_kv4_decode_supports.argtypes = [_I, _I]
     lib.cib_attention_kv4_decode_supports.restype = _I
     lib.cib_attention_kv4_decode_ctas.argtypes = [_I]
@@ -950,6 +953,21 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
         note_flagged_launch()
         _count()
         return
+    if bound or max(query_lens_host) > 1:
+        g = num_q_heads // num_kv_heads
+        if bound:
+            tiles = T * g // 64 + R
+        else:
+            tiles = sum(-(-n * g // 64) for n in query_lens_host if n >= least_query)
+        if not tiles:
+            return
+        cluster = kv4_rows_cluster(tiles * num_kv_heads, min(max_seq_len, window + max(query_lens_host) if window else max_seq_len),
+                                   148 * lib.cib_attention_kv4_rows_ctas(head_dim))
+        rc = lib.cib_attention_kv4_rows(q_args[0], dtype, q_args[1], *out_args, *cache_args, R, tiles, cluster, least_query, num_q_heads, num_kv_heads, head_dim,
+                                        float(scale), int(window), pdl, _stream())
+        _check(rc, who)
+        _count()
+        return
     rc = lib.cib_attention_kv4_generic(q_args[0], dtype, q_args[1], *out_args, *cache_args, T, R, max_seq_len, least_query, num_q_heads, num_kv_heads,
                                        head_dim, float(scale), int(window), pdl, _stream())
     _check(rc, who)
@@ -961,6 +979,15 @@ def kv4_prompt_shares(ctas: int, keys: int, values: int) -> int:
     ``keys`` keys: as many as the 148 SMs take at once, with 512 keys each at least, and while the partial results (``values`` numbers a
     share, written and read) stay below 2^24 numbers."""
     return max(1, min(148 // max(1, ctas), keys // 512, (1 << 24) // max(1, values)))
+
+
+def kv4_rows_cluster(ctas: int, keys: int, slots: int) -> int:
+    """How many CTAs (1, 2, 4 or 8) share the keys of 64 rows in the 4-bit prompt attention without tensor cores, for ``ctas`` row tiles over all key
+    heads of at most ``keys`` keys on a GPU that holds ``slots`` of its CTAs: as many as fit at once, with 128 keys each at least."""
+    cluster = 1
+    while cluster < 8 and ctas * cluster * 2 <= slots and keys > cluster * 128:
+        cluster *= 2
+    return cluster
 
 
 KV4_CLUSTER_MAX_KEYS = 1024

@@ -653,3 +653,31 @@ def test_a_table_that_is_a_part_of_a_wider_one(dtype, d, new):
     c["table"] = [row[2:6] for row in c["table"]]
     attend(c, table=wide[:, 2:6])
     check(c, c["out"])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("window", [0, 60])
+@pytest.mark.parametrize("cluster", [1, 2, 8])
+def test_prompts_without_tensor_cores(monkeypatch, dtype, d, window, cluster):
+    """Row tiles that end inside a request, a tile of a single row, single tokens among them, keys shared by none, a few or many."""
+    monkeypatch.setattr(kernels, "kv4_rows_cluster", lambda *a: cluster)
+    c = case([130, 1, 33, 300], [65, 1, 33, 1], 6, 2, d, 16, dtype, window=window, seed=d + cluster, spare_rows=2, holes=[(0, 1, -1), (3, 4, 99999)])
+    if dtype == BF16:                                                # rows that are not 16-byte aligned: no tensor cores at any head size
+        wide = torch.zeros(c["q"].shape[0], c["q"].shape[1] + 71, dtype=dtype, device=DEV)
+        wide[:, 1:1 + c["q"].shape[1]] = c["q"]
+        c["q"] = wide[:, 1:1 + c["q"].shape[1]]
+    check(c)
+
+
+@pytest.mark.parametrize("d", [96, 128])
+@pytest.mark.parametrize("requests", [1, 3, 70])
+def test_single_tokens_whose_keys_a_cluster_shares(d, requests):
+    lengths = [1500, 260, 900][:requests] if requests < 4 else [(37 * r) % 700 for r in range(requests)]
+    check(case(lengths, [1] * requests, 10, 2, d, 16, F32, seed=requests, holes=[(0, 0, -1)] if requests < 4 else ()))
+
+
+def test_how_the_keys_of_row_tiles_are_shared():
+    assert kernels.kv4_rows_cluster(1, 4000, 296) == 8 and kernels.kv4_rows_cluster(1, 128, 296) == 1
+    assert kernels.kv4_rows_cluster(148, 4000, 296) == 2 and kernels.kv4_rows_cluster(149, 4000, 296) == 1
+    assert kernels.kv4_rows_cluster(1, 257, 296) == 4
