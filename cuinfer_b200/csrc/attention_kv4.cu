@@ -22,18 +22,25 @@ constexpr int kHeads = 4;
 constexpr int kMaxWarps = 8;
 constexpr int kMaxCluster = 8;
 
-template <typename T>
+template <int N>
+struct alignas(N * 4) Words {
+    uint32_t w[N];
+};
+// code - zero (the lowest four bits of `x`): under the exponent of 2^23, less 2^23 + zero, it is exact
+__device__ __forceinline__ float less(uint32_t x, float minus) { return __uint_as_float(0x4b000000u | (x & 15u)) - minus; }
+
+template <typename T, int NG>
 __global__ void __launch_bounds__(kMaxWarps * 32)
 attention_generic_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out, int out_stride, unsigned char* __restrict__ cache, int num_pages,
                          int page_size, const int* __restrict__ block_table, int table_stride, int table_cols, const int* __restrict__ query_start_loc,
-                         const int* __restrict__ seq_lens, int num_requests, int least_query, int nq, int nkv, int d, float scale, int window, int cluster) {
-    extern __shared__ float smem[];
+                         const int* __restrict__ seq_lens, int num_requests, int least_query, int nq, int nkv, float scale, int window, int cluster) {
+    constexpr int d = kGroup * NG;
+    extern __shared__ __align__(16) float smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int t = blockIdx.x / cluster, rank = blockIdx.x - t * cluster, kvh = blockIdx.y;
     const int g = nq / nkv;
     const int head0 = kvh * g + blockIdx.z * kHeads;
     const int nh = min(kHeads, (kvh + 1) * g - head0);
-    const int groups = d / kGroup;
     griddep_wait();
     griddep_launch();
     // the request of this row: the last one that starts at or before it
@@ -54,76 +61,92 @@ attention_generic_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ 
     for (int i = threadIdx.x; i < nh * d; i += blockDim.x) qs[i] = to_f32(q[(size_t)t * q_stride + (size_t)head0 * d + i]) * scale;
     __syncthreads();
 
-    float acc[kHeads][kMaxHeadDim / kGroup];
+    float acc[kHeads][NG];
     float m[kHeads], l[kHeads];
 #pragma unroll
     for (int h = 0; h < kHeads; ++h) {
         m[h] = -INFINITY, l[h] = 0.f;
 #pragma unroll
-        for (int k = 0; k < kMaxHeadDim / kGroup; ++k) acc[h][k] = 0.f;
+        for (int k = 0; k < NG; ++k) acc[h][k] = 0.f;
     }
-    for (int c = lo + (rank * warps + warp) * 32; c <= pos; c += cluster * warps * 32) {
-        const int j = c + lane;
+    constexpr int V = NG % 4 == 0 ? 4 : NG % 2 == 0 ? 2 : 1;     // words of a load
+    for (int c = lo / 32 * 32 + (rank * warps + warp) * 32; c <= pos; c += cluster * warps * 32) {
+        const int j = c + lane;                            // lanes 0-15 have a block's keys, 16-31 the next one's
         const unsigned char* block = nullptr;
-        if (j <= pos && j / page_size < table_cols) {
-            const int page = table[j / page_size];
-            if (page >= 0 && page < num_pages) block = block_of(cache, page * page_size + j % page_size, num_pages, page_size, nkv, kvh, d);
+        if (c + (lane & 16) <= pos && (c + (lane & 16)) / page_size < table_cols) {
+            const int page = table[(c + (lane & 16)) / page_size];
+            if (page >= 0 && page < num_pages) block = block_of(cache, page * page_size + (c + (lane & 16)) % page_size, num_pages, page_size, nkv, kvh, d);
         }
-        float s[kHeads];
+        const bool seen = block != nullptr && j >= lo && j <= pos;
+        float s[kHeads] = {0.f, 0.f, 0.f, 0.f};
+        if (seen) {
+            const Words<V>* codes = reinterpret_cast<const Words<V>*>(block) + (lane & 15) * 4 * (NG / V);
+            const uint16_t* words = reinterpret_cast<const uint16_t*>(block + key_words_at(d)) + (lane & 15) * NG;
 #pragma unroll
-        for (int h = 0; h < kHeads; ++h) s[h] = block != nullptr ? 0.f : -INFINITY;
-        if (block != nullptr) {
-            const uint32_t* codes = reinterpret_cast<const uint32_t*>(block) + (j % kBlock) * 4 * groups;
-            const uint16_t* words = reinterpret_cast<const uint16_t*>(block + key_words_at(d)) + (j % kBlock) * groups;
-            for (int k = 0; k < groups; ++k) {
-                const uint32_t w = words[k];
-                const int zero = (int)(w & 15u);
-                float dot[kHeads] = {0.f, 0.f, 0.f, 0.f};
-                for (int u = 0; u < 4; ++u) {
-                    const uint32_t code = codes[u * groups + k];
+            for (int k0 = 0; k0 < NG; k0 += V) {
+                Words<V> code[4];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float x = (float)((int)((code >> (4 * (e >> 1) + 16 * (e & 1))) & 15u) - zero);
+                for (int u = 0; u < 4; ++u) code[u] = codes[u * (NG / V) + k0 / V];
 #pragma unroll
-                        for (int h = 0; h < kHeads; ++h)
-                            if (h < nh) dot[h] = fmaf(qs[h * d + k * kGroup + u * 8 + e], x, dot[h]);
+                for (int k = 0; k < V; ++k) {
+                    const uint32_t w = words[k0 + k];
+                    const float minus = 8388608.f + (float)(w & 15u), step = step_of(w);
+                    float dot[kHeads] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const uint32_t x = code[u].w[k];
+                        float v[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = less(x >> (4 * (e >> 1) + 16 * (e & 1)), minus);
+#pragma unroll
+                        for (int h = 0; h < kHeads; ++h) {
+                            if (h < nh) {
+                                const float4* qv = reinterpret_cast<const float4*>(qs + h * d + (k0 + k) * kGroup + u * 8);
+                                const float4 a = qv[0], b = qv[1];
+                                dot[h] = fmaf(a.x, v[0], fmaf(a.y, v[1], fmaf(a.z, v[2], fmaf(a.w, v[3], dot[h]))));
+                                dot[h] = fmaf(b.x, v[4], fmaf(b.y, v[5], fmaf(b.z, v[6], fmaf(b.w, v[7], dot[h]))));
+                            }
+                        }
                     }
-                }
-                const float step = step_of(w);
 #pragma unroll
-                for (int h = 0; h < kHeads; ++h) s[h] = fmaf(step, dot[h], s[h]);
+                    for (int h = 0; h < kHeads; ++h) s[h] = fmaf(step, dot[h], s[h]);
+                }
             }
         }
         float p[kHeads];
 #pragma unroll
         for (int h = 0; h < kHeads; ++h) {
-            const float top = fmaxf(m[h], warp_max(s[h]));
+            p[h] = 0.f;
+            if (h >= nh) continue;
+            const float top = fmaxf(m[h], warp_max(seen ? s[h] : -INFINITY));
             const float base = top == -INFINITY ? 0.f : top;
-            p[h] = block != nullptr ? expf(s[h] - base) : 0.f;
+            if (seen) p[h] = expf(s[h] - base);
             const float corr = m[h] == -INFINITY ? 0.f : expf(m[h] - base);
             l[h] = l[h] * corr + warp_sum(p[h]);
             m[h] = top;
 #pragma unroll
-            for (int k = 0; k < kMaxHeadDim / kGroup; ++k) acc[h][k] *= corr;
+            for (int k = 0; k < NG; ++k) acc[h][k] *= corr;
         }
-        const int count = min(32, pos - c + 1);
-        for (int jj = 0; jj < count; ++jj) {
-            const unsigned char* from = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, (unsigned long long)block, jj));
-            float pj[kHeads];
+        // values: two tokens share a word; what is not seen counts as zero, whatever lies there
+        const uint32_t mask = __ballot_sync(0xffffffffu, seen);
 #pragma unroll
-            for (int h = 0; h < kHeads; ++h) pj[h] = __shfl_sync(0xffffffffu, p[h], jj);
-            if (from == nullptr) continue;
-            const int token = (c + jj) % kBlock;
-            const uint16_t* words = reinterpret_cast<const uint16_t*>(from + value_words_at(d)) + (token >> 1) * groups * 2 + (token & 1);
-            const uint16_t* codes = reinterpret_cast<const uint16_t*>(from + value_codes_at(d)) +
-                                    (size_t)(((token >> 3) * 8 + (lane >> 2)) * 4 + ((token & 7) >> 1)) * groups * 2 + (token & 1);
+        for (int b = 0; b < 2; ++b) {
+            const unsigned char* from = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, (unsigned long long)block, 16 * b));
+            if (((mask >> (16 * b)) & 0xffffu) == 0) continue;
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(from + value_words_at(d));
+            const uint32_t* codes = reinterpret_cast<const uint32_t*>(from + value_codes_at(d)) + (lane >> 2) * 4 * NG;
+#pragma unroll 4
+            for (int i = 0; i < 8; ++i) {                  // tokens 2 i and 2 i + 1
+                const uint32_t two = mask >> (16 * b + 2 * i), keep = (two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
+                float p0[kHeads], p1[kHeads];
 #pragma unroll
-            for (int k = 0; k < kMaxHeadDim / kGroup; ++k) {
-                if (k < groups) {
-                    const uint32_t w = words[2 * k];
-                    const float x = step_of(w) * (float)((int)((codes[2 * k] >> (4 * (lane & 3))) & 15u) - (int)(w & 15u));
+                for (int h = 0; h < kHeads; ++h) p0[h] = __shfl_sync(0xffffffffu, p[h], 16 * b + 2 * i), p1[h] = __shfl_sync(0xffffffffu, p[h], 16 * b + 2 * i + 1);
 #pragma unroll
-                    for (int h = 0; h < kHeads; ++h) acc[h][k] = fmaf(pj[h], x, acc[h][k]);
+                for (int k = 0; k < NG; ++k) {
+                    const uint32_t w = words[i * NG + k] & keep, x = codes[((i >> 2) * 32 + (i & 3)) * NG + k] >> (4 * (lane & 3));
+                    const float x0 = less(x, 8388608.f + (float)(w & 15u)) * step_of(w), x1 = less(x >> 16, 8388608.f + (float)((w >> 16) & 15u)) * step_of(w >> 16);
+#pragma unroll
+                    for (int h = 0; h < kHeads; ++h) acc[h][k] = fmaf(p0[h], x0, fmaf(p1[h], x1, acc[h][k]));
                 }
             }
         }
@@ -135,8 +158,7 @@ attention_generic_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ 
     for (int h = 0; h < kHeads; ++h) {
         float* mine = part + (size_t)(warp * kHeads + h) * (d + 2);
 #pragma unroll
-        for (int k = 0; k < kMaxHeadDim / kGroup; ++k)
-            if (k < groups) mine[k * kGroup + lane] = acc[h][k];
+        for (int k = 0; k < NG; ++k) mine[k * kGroup + lane] = acc[h][k];
         if (lane == 0) mine[d] = m[h], mine[d + 1] = l[h];
     }
     __syncthreads();
@@ -209,15 +231,25 @@ extern "C" int cib_attention_kv4_generic(const void* q, int dtype, int q_stride,
     const size_t smem = (size_t)(kv4::kHeads * d + (warps + (cluster > 1 ? 1 : 0)) * kv4::kHeads * (d + 2)) * sizeof(float);
     CIB_REQUIRE((long long)num_tokens * cluster < (1ll << 31), "attention_kv4: too many rows");
     const dim3 grid(num_tokens * cluster, nkv, (g + kv4::kHeads - 1) / kv4::kHeads);
-    cudaError_t e;
-    if (dtype == kF32)
-        e = launch_pdl_cluster(kv4::attention_generic_kernel<float>, grid, dim3(warps * 32), smem, stream, use_pdl != 0, cluster, (const float*)q, q_stride, (float*)out, out_stride,
-                       (unsigned char*)cache, num_pages, page_size, block_table, table_stride, table_cols, query_start_loc, seq_lens, num_requests, least_query, nq, nkv, d,
-                       scale, window, cluster);
-    else
-        e = launch_pdl_cluster(kv4::attention_generic_kernel<__nv_bfloat16>, grid, dim3(warps * 32), smem, stream, use_pdl != 0, cluster, (const __nv_bfloat16*)q, q_stride,
-                       (__nv_bfloat16*)out, out_stride, (unsigned char*)cache, num_pages, page_size, block_table, table_stride, table_cols, query_start_loc, seq_lens,
-                       num_requests, least_query, nq, nkv, d, scale, window, cluster);
+    cudaError_t e = cudaErrorInvalidValue;
+#define CIB_KV4_SINGLE(NGV)                                                                                                                                \
+    if (d == 32 * NGV && dtype == kF32)                                                                                                                    \
+        e = launch_pdl_cluster(kv4::attention_generic_kernel<float, NGV>, grid, dim3(warps * 32), smem, stream, use_pdl != 0, cluster, (const float*)q, q_stride, \
+                               (float*)out, out_stride, (unsigned char*)cache, num_pages, page_size, block_table, table_stride, table_cols, query_start_loc,    \
+                               seq_lens, num_requests, least_query, nq, nkv, scale, window, cluster);                                                         \
+    if (d == 32 * NGV && dtype == kBF16)                                                                                                                   \
+        e = launch_pdl_cluster(kv4::attention_generic_kernel<__nv_bfloat16, NGV>, grid, dim3(warps * 32), smem, stream, use_pdl != 0, cluster,                 \
+                               (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, (unsigned char*)cache, num_pages, page_size, block_table,    \
+                               table_stride, table_cols, query_start_loc, seq_lens, num_requests, least_query, nq, nkv, scale, window, cluster)
+    CIB_KV4_SINGLE(1);
+    CIB_KV4_SINGLE(2);
+    CIB_KV4_SINGLE(3);
+    CIB_KV4_SINGLE(4);
+    CIB_KV4_SINGLE(5);
+    CIB_KV4_SINGLE(6);
+    CIB_KV4_SINGLE(7);
+    CIB_KV4_SINGLE(8);
+#undef CIB_KV4_SINGLE
     CIB_REQUIRE(e == cudaSuccess, "attention_kv4: launch failed: %s", cudaGetErrorString(e));
     return 0;
 }

@@ -25,6 +25,28 @@ namespace kv4r {
 
 using namespace kv4;
 
+// two 32-bit multiply-adds at a time; {a, b} of two neighbouring registers
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 both(uint64_t a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 constexpr int kRows = 64, kKeys = 32, kWarps = 8, kCluster = 8;
 
 template <int NG>
@@ -178,13 +200,14 @@ attention_rows_kernel(const void* __restrict__ q, int bf16, int q_stride, void* 
         pos[i] = grow < rows_total ? seq_len - n + grow / g : -1;
     }
     const int warp_first = seq_len - n + (row0 + 8 * warp) / g, warp_last = row0 + 8 * warp + 7 < rows_total ? seq_len - n + (row0 + 8 * warp + 7) / g : 0x7fffffff;
-    float m[4], l[4], acc[8][NG];
+    float m[4], l[4];
+    uint64_t acc[4][NG];                                         // rows 2 i and 2 i + 1
 #pragma unroll
     for (int i = 0; i < 4; ++i) m[i] = -INFINITY, l[i] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int k = 0; k < NG; ++k) acc[i][k] = 0.f;
+        for (int k = 0; k < NG; ++k) acc[i][k] = 0;
     const float* qr = sQ + (8 * warp + 4 * rg) * P;
     const float* kr = sK + ki * P;
     float* pw = sP + warp * kKeys * 8;
@@ -199,18 +222,22 @@ attention_rows_kernel(const void* __restrict__ q, int bf16, int q_stride, void* 
         }
         if (!live) continue;
         const int key0 = k0 + j * kKeys;
-        float s[4][2];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[i][0] = s[i][1] = 0.f;
+        uint64_t sums[4][2] = {};                                // of even and odd columns
 #pragma unroll 4
         for (int c = 0; c < D; c += 4) {
-            const float4 a = *reinterpret_cast<const float4*>(kr + c), b = *reinterpret_cast<const float4*>(kr + 16 * P + c);
+            const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(kr + c), b = *reinterpret_cast<const ulonglong2*>(kr + 16 * P + c);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float4 x = *reinterpret_cast<const float4*>(qr + i * P + c);
-                s[i][0] = fmaf(x.x, a.x, fmaf(x.y, a.y, fmaf(x.z, a.z, fmaf(x.w, a.w, s[i][0]))));
-                s[i][1] = fmaf(x.x, b.x, fmaf(x.y, b.y, fmaf(x.z, b.z, fmaf(x.w, b.w, s[i][1]))));
+                const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(qr + i * P + c);
+                sums[i][0] = fma2(x.y, a.y, fma2(x.x, a.x, sums[i][0]));
+                sums[i][1] = fma2(x.y, b.y, fma2(x.x, b.x, sums[i][1]));
             }
+        }
+        float s[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 a = both(sums[i][0]), b = both(sums[i][1]);
+            s[i][0] = a.x + a.y, s[i][1] = b.x + b.y;
         }
         const bool whole = s_named[0] && s_named[1] && key0 + kKeys - 1 <= warp_first && (window <= 0 || (warp_last != 0x7fffffff && key0 > warp_last - window));
         uint32_t seen = 0xffu;                                   // of key `lane`: which of the warp's eight rows see it
@@ -245,10 +272,11 @@ attention_rows_kernel(const void* __restrict__ q, int bf16, int q_stride, void* 
         }
         if (__any_sync(0xffffffffu, changes)) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float f = __shfl_sync(0xffffffffu, corr[i & 3], (i >> 2) * 16);
+            for (int i = 0; i < 4; ++i) {
+                const int from = (i >> 1) * 16;
+                const uint64_t f = pair_of(__shfl_sync(0xffffffffu, corr[2 * (i & 1)], from), __shfl_sync(0xffffffffu, corr[2 * (i & 1) + 1], from));
 #pragma unroll
-                for (int k = 0; k < NG; ++k) acc[i][k] *= f;
+                for (int k = 0; k < NG; ++k) acc[i][k] = mul2(acc[i][k], f);
             }
         }
         *reinterpret_cast<float4*>(pw + ki * 8 + 4 * rg) = make_float4(s[0][0], s[1][0], s[2][0], s[3][0]);
@@ -257,13 +285,15 @@ attention_rows_kernel(const void* __restrict__ q, int bf16, int q_stride, void* 
         if (whole) {
 #pragma unroll 4
             for (int x = 0; x < kKeys; ++x) {
-                const float4 a = *reinterpret_cast<const float4*>(pw + x * 8), b = *reinterpret_cast<const float4*>(pw + x * 8 + 4);
-                const float p[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(pw + x * 8), b = *reinterpret_cast<const ulonglong2*>(pw + x * 8 + 4);
 #pragma unroll
                 for (int k = 0; k < NG; ++k) {
                     const float v = sV[x * P + kGroup * k + lane];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) acc[i][k] = fmaf(p[i], v, acc[i][k]);
+                    const uint64_t vv = pair_of(v, v);
+                    acc[0][k] = fma2(a.x, vv, acc[0][k]);
+                    acc[1][k] = fma2(a.y, vv, acc[1][k]);
+                    acc[2][k] = fma2(b.x, vv, acc[2][k]);
+                    acc[3][k] = fma2(b.y, vv, acc[3][k]);
                 }
             }
         } else {
@@ -276,8 +306,10 @@ attention_rows_kernel(const void* __restrict__ q, int bf16, int q_stride, void* 
                 for (int k = 0; k < NG; ++k) {
                     const float v = sV[x * P + kGroup * k + lane];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if ((rows >> i) & 1u) acc[i][k] = fmaf(p[i], v, acc[i][k]);
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 o = both(acc[i][k]);
+                        acc[i][k] = pair_of((rows >> (2 * i)) & 1u ? fmaf(p[2 * i], v, o.x) : o.x, (rows >> (2 * i + 1)) & 1u ? fmaf(p[2 * i + 1], v, o.y) : o.y);
+                    }
                 }
             }
         }
@@ -301,7 +333,7 @@ attention_rows_kernel(const void* __restrict__ q, int bf16, int q_stride, void* 
             const float sum = __shfl_sync(0xffffffffu, l[i & 3], (i >> 2) * 16);
             if (row0 + 8 * warp + i < rows_total) {
 #pragma unroll
-                for (int k = 0; k < NG; ++k) store(8 * warp + i, kGroup * k + lane, sum, acc[i][k]);
+                for (int k = 0; k < NG; ++k) store(8 * warp + i, kGroup * k + lane, sum, i & 1 ? both(acc[i >> 1][k]).y : both(acc[i >> 1][k]).x);
             }
         }
         return;
@@ -310,7 +342,7 @@ attention_rows_kernel(const void* __restrict__ q, int bf16, int q_stride, void* 
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int k = 0; k < NG; ++k) sQ[(8 * warp + i) * P + kGroup * k + lane] = acc[i][k];
+        for (int k = 0; k < NG; ++k) sQ[(8 * warp + i) * P + kGroup * k + lane] = i & 1 ? both(acc[i >> 1][k]).y : both(acc[i >> 1][k]).x;
     if (ki == 0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) sML[(8 * warp + 4 * rg + i) * 2] = m[i], sML[(8 * warp + 4 * rg + i) * 2 + 1] = l[i];
