@@ -1,14 +1,15 @@
 // Prompt attention over the cache that is held in 4 bits (kv4.cuh) without tensor cores: any head size that is a multiple of 32 up to 256, any head
-// counts, 32-bit queries, and bfloat16 ones of the head sizes and alignments that the tensor-core kernel does not take.
+// counts, 32-bit queries, and bfloat16 ones whose rows are not 16-byte aligned.
 //
 //   out = softmax(scale * q K^T over the keys position - window < j <= position) V,  32-bit multiply-adds throughout, the exact exponential
 //
 // A CTA has 64 rows (query token x query head of one kv head) of one request and walks tiles of 32 keys: half of its threads take the tile's keys
 // apart and half its values, into shared memory as 32-bit numbers, from words that were asked for a tile ahead, so a code is taken apart once for
-// 64 rows (a token at a time, four heads for a code, 2 x 400 tokens behind 1 600, 8 heads of 256, took 1 597 us).  A warp has eight rows: a lane
-// computes the scores of four of them with two keys (32 multiply-adds for 6 loads of 16 bytes), the warp takes the exponentials of its own
+// 64 rows (a token at a time, four heads for a code, a prompt of 400 tokens, 16 heads over 8 of 128, took 263 us, 90 so).  A warp has eight rows: a lane
+// computes the scores of four of them with two keys (32 multiply-adds, two to an instruction, for 6 loads of 16 bytes), the warp takes the exponentials of its own
 // scores and passes them to itself as the weights of the sum of the values, of which a lane has every 32nd column: 8 D / 32 sums in registers.  Nothing
-// but the tile is exchanged between warps.  Bound by the multiply-adds and the shared memory's reads, about alike.
+// but the tile is exchanged between warps.  Bound by latency: with 8 heads of 256 issue slots are 0.39 busy, the multiply-add pipe 0.25 and shared memory 0.39
+// (two warps a scheduler; their registers hold the sums).
 //
 // Where a launch would leave SMs without work, a cluster of up to eight CTAs shares the key tiles of 64 rows; the partial results are joined through
 // distributed shared memory.

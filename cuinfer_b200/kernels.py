@@ -123,6 +123,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "cib_kv4_read": [_P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
         "cib_attention_kv4_generic": [_P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
         "cib_attention_kv4_rows": [_P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
+        "cib_attention_kv4_rows_mma": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
         "cib_attention_kv4_prompt": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P],
         "cib_attention_kv4_decode": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _I, _P, _P, _I, _P],
         "cib_gemm_skinny": [_P, _I, _I, _I, _P, _I, _P, _P, _I, _P, _I, _F, _P, _P, _I, _I, _I, _I, _I, _P, ctypes.c_longlong, _P, _I, _P, _P, _P],
@@ -961,8 +962,15 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
             tiles = sum(-(-n * g // 64) for n in query_lens_host if n >= least_query)
         if not tiles:
             return
+        mma = dtype == BF16 and q_args[1] % 8 == 0 and q_args[0] % 16 == 0
         cluster = kv4_rows_cluster(tiles * num_kv_heads, min(max_seq_len, window + max(query_lens_host) if window else max_seq_len),
-                                   148 * lib.cib_attention_kv4_rows_ctas(head_dim))
+                                   148 * (2 if mma else lib.cib_attention_kv4_rows_ctas(head_dim)))
+        if mma:
+            rc = lib.cib_attention_kv4_rows_mma(*q_args, *out_args, *cache_args, R, tiles, cluster, least_query, num_q_heads, num_kv_heads, head_dim,
+                                                float(scale), int(window), pdl, _stream())
+            _check(rc, who)
+            _count()
+            return
         rc = lib.cib_attention_kv4_rows(q_args[0], dtype, q_args[1], *out_args, *cache_args, R, tiles, cluster, least_query, num_q_heads, num_kv_heads, head_dim,
                                         float(scale), int(window), pdl, _stream())
         _check(rc, who)

@@ -681,3 +681,12 @@ def test_how_the_keys_of_row_tiles_are_shared():
     assert kernels.kv4_rows_cluster(1, 4000, 296) == 8 and kernels.kv4_rows_cluster(1, 128, 296) == 1
     assert kernels.kv4_rows_cluster(148, 4000, 296) == 2 and kernels.kv4_rows_cluster(149, 4000, 296) == 1
     assert kernels.kv4_rows_cluster(1, 257, 296) == 4
+
+
+@pytest.mark.parametrize("d", [32, 96, 160, 192, 224, 256])
+@pytest.mark.parametrize("window", [0, 60])
+@pytest.mark.parametrize("cluster", [1, 2, 8])
+def test_prompts_of_head_sizes_between(monkeypatch, d, window, cluster):
+    monkeypatch.setattr(kernels, "kv4_rows_cluster", lambda *a: cluster)
+    check(case([130, 1, 33, 300], [65, 1, 33, 1], 6, 2, d, 16, BF16, window=window, seed=d + cluster, spare_rows=2, holes=[(0, 1, -1), (3, 4, 99999)]))
+    check(case([400, 90], [31, 90], 9, 1, d, 48, BF16, window=window, seed=d, spare_rows=1))
