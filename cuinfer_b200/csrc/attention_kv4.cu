@@ -33,7 +33,7 @@ template <typename T, int NG>
 __global__ void __launch_bounds__(kMaxWarps * 32)
 attention_generic_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out, int out_stride, unsigned char* __restrict__ cache, int num_pages,
                          int page_size, const int* __restrict__ block_table, int table_stride, int table_cols, const int* __restrict__ query_start_loc,
-                         const int* __restrict__ seq_lens, int num_requests, int least_query, int nq, int nkv, float scale, int window, int cluster) {
+                         const int* __restrict__ seq_lens, int num_requests, int nq, int nkv, float scale, int window, int cluster) {
     constexpr int d = kGroup * NG;
     extern __shared__ __align__(16) float smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
@@ -52,7 +52,6 @@ attention_generic_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ 
     const int r = before - 1;
     if (r < 0 || r >= num_requests) return;
     const int q0 = query_start_loc[r], n = query_start_loc[r + 1] - q0;
-    if (n < least_query) return;
     const int pos = seq_lens[r] - n + (t - q0);
     const int lo = window > 0 ? max(0, pos - window + 1) : 0;
     const int* table = block_table + (size_t)r * table_stride;
@@ -205,10 +204,9 @@ attention_generic_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ 
 using namespace cib;
 
 // query_start_loc holds num_requests + 1 boundaries of the num_tokens rows.  longest: no request has more keys (it shapes the launch only).
-// least_query: rows of requests that bring fewer tokens are left as they are.
 extern "C" int cib_attention_kv4_generic(const void* q, int dtype, int q_stride, void* out, int out_stride, const void* cache, int num_pages, int page_size,
                                          const int* block_table, int table_stride, int table_cols, const int* query_start_loc, const int* seq_lens, int num_tokens,
-                                         int num_requests, int longest, int least_query, int nq, int nkv, int d, float scale, int window, int use_pdl,
+                                         int num_requests, int longest, int nq, int nkv, int d, float scale, int window, int use_pdl,
                                          cudaStream_t stream) {
     CIB_REQUIRE(num_tokens >= 0 && nq > 0 && nkv > 0 && nq % nkv == 0, "attention_kv4: bad sizes T=%d nq=%d nkv=%d", num_tokens, nq, nkv);
     CIB_REQUIRE(kv4::sizes_ok(d, page_size), "attention_kv4: head size %d must be a multiple of 32 up to 256, page size %d a multiple of 16", d, page_size);
@@ -236,11 +234,11 @@ extern "C" int cib_attention_kv4_generic(const void* q, int dtype, int q_stride,
     if (d == 32 * NGV && dtype == kF32)                                                                                                                    \
         e = launch_pdl_cluster(kv4::attention_generic_kernel<float, NGV>, grid, dim3(warps * 32), smem, stream, use_pdl != 0, cluster, (const float*)q, q_stride, \
                                (float*)out, out_stride, (unsigned char*)cache, num_pages, page_size, block_table, table_stride, table_cols, query_start_loc,    \
-                               seq_lens, num_requests, least_query, nq, nkv, scale, window, cluster);                                                         \
+                               seq_lens, num_requests, nq, nkv, scale, window, cluster);                                                         \
     if (d == 32 * NGV && dtype == kBF16)                                                                                                                   \
         e = launch_pdl_cluster(kv4::attention_generic_kernel<__nv_bfloat16, NGV>, grid, dim3(warps * 32), smem, stream, use_pdl != 0, cluster,                 \
                                (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, (unsigned char*)cache, num_pages, page_size, block_table,    \
-                               table_stride, table_cols, query_start_loc, seq_lens, num_requests, least_query, nq, nkv, scale, window, cluster)
+                               table_stride, table_cols, query_start_loc, seq_lens, num_requests, nq, nkv, scale, window, cluster)
     CIB_KV4_SINGLE(1);
     CIB_KV4_SINGLE(2);
     CIB_KV4_SINGLE(3);

@@ -121,7 +121,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "cib_attention_tcgen05": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P],
         "cib_qk_norm_rope_kv4_write": [_P, _I, _I, _P, _I, _P, _P, _P, _P, _I, _I, _F, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P],
         "cib_kv4_read": [_P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
-        "cib_attention_kv4_generic": [_P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
+        "cib_attention_kv4_generic": [_P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
         "cib_attention_kv4_rows": [_P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
         "cib_attention_kv4_rows_mma": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
         "cib_attention_kv4_prompt": [_P, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P],
@@ -932,7 +932,7 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
         _check(rc, who)
         note_flagged_launch()
         _count()
-        if T <= R and max(query_lens_host) <= 1:                # (nothing but single tokens)
+        if max(query_lens_host) <= 1:                           # (nothing but single tokens)
             return
         least_query = 2
     if (dtype == BF16 and lib.cib_attention_kv4_prompt_supports(head_dim, page_size) and scale > 0
@@ -954,7 +954,7 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
         note_flagged_launch()
         _count()
         return
-    if bound or max(query_lens_host) > 1:
+    if max(query_lens_host) > 1:
         g = num_q_heads // num_kv_heads
         if bound:
             tiles = T * g // 64 + R
@@ -976,7 +976,7 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
         _check(rc, who)
         _count()
         return
-    rc = lib.cib_attention_kv4_generic(q_args[0], dtype, q_args[1], *out_args, *cache_args, T, R, max_seq_len, least_query, num_q_heads, num_kv_heads,
+    rc = lib.cib_attention_kv4_generic(q_args[0], dtype, q_args[1], *out_args, *cache_args, T, R, max_seq_len, num_q_heads, num_kv_heads,
                                        head_dim, float(scale), int(window), pdl, _stream())
     _check(rc, who)
     _count()

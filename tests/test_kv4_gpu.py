@@ -690,3 +690,12 @@ def test_prompts_of_head_sizes_between(monkeypatch, d, window, cluster):
     monkeypatch.setattr(kernels, "kv4_rows_cluster", lambda *a: cluster)
     check(case([130, 1, 33, 300], [65, 1, 33, 1], 6, 2, d, 16, BF16, window=window, seed=d + cluster, spare_rows=2, holes=[(0, 1, -1), (3, 4, 99999)]))
     check(case([400, 90], [31, 90], 9, 1, d, 48, BF16, window=window, seed=d, spare_rows=1))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [64, 96, 256])
+def test_single_tokens_with_rows_behind_them_and_requests_without(dtype, d):
+    """More rows than requests, and more requests than rows (as a padded step has): rows behind the last request stay."""
+    check(case([40, 300, 17], [1, 1, 1], 4, 2, d, 16, dtype, seed=d, spare_rows=5))
+    c = case([40, 300, 17, 0, 0], [1, 1, 1, 0, 0], 4, 2, d, 16, dtype, seed=d)
+    check(c, attend(c, lens=[1] * 5))
