@@ -148,8 +148,8 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
     uint64_t* pv_done = bars + 12;      // [row tile][2] O includes a key tile: its values' buffer is free
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
     __shared__ int s_req, s_pair, s_abort, s_q0, s_n, s_seq;
-    // Which of a key tile's blocks the table does not name, tile j at j % 4: written when S of tile j - 2 is there, so P V of tile j - 4 was issued and
-    // every row is through with that tile.
+    // Which of a key tile's blocks the table does not name, tile j at j % 4: written when every row is through with tile j - 4.  Of a row tile that
+    // walks tile j - 2 its S says so (P V of tile j - 4 was issued before it); of one that ends earlier, P of tile j - 4.
     __shared__ int s_missing[4];
     __shared__ int s_odd;               // a value that is not a number has been met
 
@@ -366,6 +366,12 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
                 const Codes x = next;
                 if (j + 1 < most) next = load(j + 1);
                 if (!free_again(s_full, j, 55)) break;
+                // a row tile that has no tile j - 2 any more may still be at its last two (no later phase of these barriers follows)
+                bool through = true;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    if (j - 4 >= 0 && j - 4 < tiles[t] && j - 2 >= tiles[t]) through = through && wait_all(&p_ready[2 * t + b], (uint32_t)((j >> 1) & 1), 63);
+                if (!through) break;
                 if (lane == 0) {
                     if (x.id < 0 && k_lo + j * kN + take * kBlock < seq_len) atomicOr(&s_missing[j & 3], 1 << take);
                     else atomicAnd(&s_missing[j & 3], ~(1 << take));
