@@ -7,18 +7,20 @@ import pytest
 import torch
 
 import plain_kv4_tight as tight
+import test_kv4_gpu as first
 from cuinfer_b200 import kernels
-from test_kv4_gpu import BF16, DEV, F32, attend, case
+from test_kv4_gpu import BF16, F32, attend, case
 
 pytestmark = pytest.mark.gpu
 
 
-def check(c, out=None, codes=True):
+def check(c, out=None):
     """Against attention in 64 bits, within what the kernels' arithmetic may be off; rows behind the last request stay."""
     out = attend(c) if out is None else out
     kernels.check_error_flags(force=True)
+    aligned = c["q"].data_ptr() % 16 == 0 and c["q"].stride(0) % 8 == 0
     want, allowed = tight.attention(c["q"], c["cache"], c["table"], c["starts"], c["lengths"], c["nq"], c["nkv"], c["d"], c["scale"], c["window"],
-                                    rounded=c["q"].dtype == BF16, codes=codes and c["d"] in (64, 128, 256))
+                                    rounded=c["q"].dtype == BF16, codes=aligned and c["d"] in (64, 128, 256))
     rows = c["starts"][-1]
     off = tight.worst(out, want, allowed, rows)
     print(f"{off:.3f} of what is allowed")
@@ -40,3 +42,89 @@ def test_pages_that_are_none_in_tiles_that_one_row_tile_no_longer_walks(monkeypa
     check(c, first)
     for _ in range(20):
         assert torch.equal(attend(c, torch.full_like(first, 5.0)), first)
+
+
+# ---- the first tests' calls, within the bound of the kernels' arithmetic ------------------------------------------------------
+
+@pytest.fixture
+def within_the_bound(monkeypatch):
+    monkeypatch.setattr(first, "check", check)
+
+
+BOTH = pytest.mark.parametrize("dtype", [F32, BF16])
+HEADS = pytest.mark.parametrize("heads", first.HEADS + [(4, 2, 192), (3, 1, 224), (4, 4, 256)])
+
+
+@BOTH
+@HEADS
+def test_single_tokens(within_the_bound, dtype, heads):
+    first.test_attention_of_single_tokens(dtype, heads, 48)
+
+
+@BOTH
+@HEADS
+def test_prompts_and_mixed_steps(within_the_bound, dtype, heads):
+    first.test_attention_of_prompts_and_mixed_steps(dtype, heads)
+
+
+@BOTH
+@pytest.mark.parametrize("window", [1, 33, 100])
+@pytest.mark.parametrize("heads", [(4, 2, 128), (6, 2, 64), (2, 1, 96), (2, 1, 256)])
+def test_windows(within_the_bound, dtype, window, heads):
+    first.test_attention_in_a_window(dtype, window, heads)
+
+
+@BOTH
+@pytest.mark.parametrize("d", [64, 128, 96, 256])
+def test_long_contexts(within_the_bound, dtype, d):
+    first.test_attention_of_long_contexts(dtype, d)
+
+
+@BOTH
+@pytest.mark.parametrize("d", [64, 128, 96, 256])
+@pytest.mark.parametrize("new", [1, 20])
+def test_holes_and_empty_rows(within_the_bound, dtype, d, new):
+    first.test_pages_that_are_none_rows_without_keys_and_empty_requests(dtype, d, new)
+
+
+@pytest.mark.parametrize("heads", [(2, 1, 128), (12, 4, 64), (5, 1, 128)])
+@pytest.mark.parametrize("shape", ["one long", "many", "portions", "bounds"])
+def test_many_row_tiles(within_the_bound, heads, shape):
+    first.test_prompts_of_many_row_tiles(heads, shape)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 300])
+@pytest.mark.parametrize("shape", [(1, 0, 0), (8, 0, 0), (0, 5, 0), (0, 3, 8), (0, 592, 8)])
+def test_shared_keys_of_single_tokens(within_the_bound, monkeypatch, d, window, shape):
+    first.test_every_way_to_share_the_keys_of_single_tokens(monkeypatch, d, window, shape)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window", [0, 150])
+@pytest.mark.parametrize("shares", [2, 9])
+def test_shared_keys_of_prompts(within_the_bound, monkeypatch, d, window, shares):
+    first.test_prompts_whose_keys_are_shared(monkeypatch, d, window, shares)
+
+
+@BOTH
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("cluster", [1, 8])
+def test_without_tensor_cores(within_the_bound, monkeypatch, dtype, d, cluster):
+    first.test_prompts_without_tensor_cores(monkeypatch, dtype, d, 0 if cluster == 1 else 60, cluster)
+
+
+@pytest.mark.parametrize("d", [32, 96, 160, 192, 224, 256])
+@pytest.mark.parametrize("cluster", [1, 8])
+def test_head_sizes_between(within_the_bound, monkeypatch, d, cluster):
+    first.test_prompts_of_head_sizes_between(monkeypatch, d, 0 if cluster == 1 else 60, cluster)
+
+
+@pytest.mark.parametrize("d", [96, 128])
+@pytest.mark.parametrize("requests", [1, 3, 70])
+def test_clusters_of_single_tokens(within_the_bound, d, requests):
+    first.test_single_tokens_whose_keys_a_cluster_shares(d, requests)
+
+
+def test_scales_that_are_not_positive(within_the_bound):
+    first.test_a_scale_that_is_not_positive()
