@@ -13,8 +13,8 @@
 // operand as they stand: a code masked out of bits 0-3 is c 2^-133, out of bits 4-7 16 c 2^-133, and one shift by 8 serves
 // the other two: 5 operations for 8 codes, where placing each code under an exponent took 7.  The queries are multiplied by a power of
 // two a head, so that their largest lies in [2^126, 2^127), and by 1/16 against the codes of bits 4-7; the scores take it back.
-// The zero points of all groups are one more MMA with step * zero (four bits times four) against the sums of q, which are split into
-// bfloat16 parts.  All operands of the scores are exact.  For the values one fused multiply-add on the other pipe gives (code - zero) 2^-6,
+// The zero points of all groups are one more MMA (two at head size 256) with step * zero (four bits times four) against the sums of q, which are
+// split into four bfloat16 parts.  All operands of the scores are exact.  For the values one fused multiply-add on the other pipe gives (code - zero) 2^-6,
 // also exact; only p * step is rounded, once: p enters that product as two bfloat16 parts.  The weights come out of the scores with keys as rows
 // and go in with keys as the summed index: an 8 x 8 transposition in registers (movmatrix) for 8 keys and part.
 //
@@ -270,9 +270,10 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
     const int exponent = largest > 1.1754944e-38f && largest < INFINITY ? (int)(__float_as_uint(largest) >> 23) - 127 : 0;
     const float down = __uint_as_float((uint32_t)(127 - exponent) << 23), tiny = exponent == 127 ? 5.877472e-39f : down;
     // minus half the sums of the scaled queries in bfloat16 parts: the B operand of the zero points.  The summed index runs over (part,
-    // group pair): quads hold part quad / kPairs of a pair, then the parts behind those.
-    uint32_t sums0 = 0, sums1 = 0;
-    constexpr int kPairs = NG / 2;
+    // group pair): quads hold part quad / kPairs of a pair, then the parts behind those.  Four pairs leave room for two parts in an MMA, which
+    // are 16 bits of a sum that may have 24: their last two parts are an MMA of their own.
+    constexpr int kPairs = NG / 2, kSums = kPairs == 4 ? 4 : 2;
+    uint32_t sums[kSums] = {};
     const int my_pair = quad % kPairs;
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
@@ -299,8 +300,9 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
             const int p0 = quad / kPairs, p1 = kFirst + p0;
             const uint32_t a = p0 == 0 ? part[0] : p0 == 1 ? part[1] : p0 == 2 ? part[2] : part[3];
             const uint32_t b = p1 == 1 ? part[1] : p1 == 2 ? part[2] : p1 == 3 ? part[3] : 0u;
-            sums0 |= a << (16 * (k & 1));
-            sums1 |= b << (16 * (k & 1));
+            sums[0] |= a << (16 * (k & 1));
+            sums[1] |= b << (16 * (k & 1));
+            if constexpr (kSums == 4) sums[2] |= part[2] << (16 * (k & 1)), sums[3] |= part[3] << (16 * (k & 1));
         }
     }
     // a sum of products stands for 2^(-7 - e) of the score; of heads 2 quad and 2 quad + 1 (column c is held by lanes 4 c ..)
@@ -336,7 +338,8 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
                 const uint32_t a = words[row * kPairs + my_pair], c = words[(row + 8) * kPairs + my_pair];
                 const uint32_t za = mul_bf16x2(mul_bf16x2(a & 0x000f000fu, k2p127), a & 0xfff0fff0u);
                 const uint32_t zc = mul_bf16x2(mul_bf16x2(c & 0x000f000fu, k2p127), c & 0xfff0fff0u);
-                mma16816_0(s[b], za, zc, za, zc, sums0, sums1);
+                mma16816_0(s[b], za, zc, za, zc, sums[0], sums[1]);
+                if constexpr (kSums == 4) mma16816(s[b], za, zc, za, zc, sums[2], sums[3]);
             }
 #pragma unroll
             for (int k = 0; k < NG; ++k) {

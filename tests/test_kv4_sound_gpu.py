@@ -3,9 +3,11 @@ from __future__ import annotations
 
 import random
 
+import numpy as np
 import pytest
 import torch
 
+import plain_kv4 as P4
 import plain_kv4_tight as tight
 import test_kv4_gpu as first
 from cuinfer_b200 import kernels
@@ -128,3 +130,37 @@ def test_clusters_of_single_tokens(within_the_bound, d, requests):
 
 def test_scales_that_are_not_positive(within_the_bound):
     first.test_a_scale_that_is_not_positive()
+
+
+# ---- scores that differ by what the sums of the queries have in their lowest bits -----------------------------------------------
+
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("new", [1, 3])
+def test_scores_of_far_zero_points(d, new):
+    """Two keys that are zero, one with codes and zero points of 15 and one of 0, under a query whose group's sum has 19 bits: both scores are
+    exactly zero.  In units of a step every product is a multiple of 2^-10 and every sum below 2^12, so none of 24 bits is cut; the weights are equal,
+    and the result is the values' mean, rounded once (2^-8) after weights of one."""
+    groups = d // 32
+    c = case([new + 1] * groups, [new] * groups, 1, 1, d, 16, BF16, seed=d)
+    c["scale"] = 4.0
+    q = torch.zeros_like(c["q"])
+    for r in range(groups):
+        q[c["starts"][r]:c["starts"][r + 1], 32 * r + 3], q[c["starts"][r]:c["starts"][r + 1], 32 * r + 14] = 258.0, 129 / 256
+        q[c["starts"][r]:c["starts"][r + 1], 32 * r + 29] = 2.0 ** -10
+    c["q"] = q
+    raw = c["cache"].cpu().numpy()
+    places = np.array(P4._places(d))[:, :, 0]
+    for r in range(groups):
+        block = raw[c["table"][r][0], 0, 0]
+        for token in range(new + 1):
+            code = 15 if token % 2 == 0 else 0
+            for byte, shift, word in places[token]:
+                block[byte] = block[byte] & ~(15 << shift) & 255 | code << shift
+                block[word], block[word + 1] = 0x80 | code, 0x42             # a step of 64
+    c["cache"] = torch.from_numpy(raw).to(first.DEV)
+    out = attend(c).double().cpu()
+    values = P4.unpack(c["cache"], d)[1]
+    for r in range(groups):
+        for i in range(new):
+            want = values[c["table"][r][0], 0, :i + 2].mean(0)
+            assert ((out[c["starts"][r] + i] - want).abs() <= 2.0 ** -8 * 1.01 * (want.abs() + (values[c["table"][r][0], 0, :i + 2].abs().mean(0) if new > 1 else 0))).all(), (r, i)
