@@ -126,8 +126,10 @@ struct alignas(sizeof(T) * E > 16 ? 16 : sizeof(T) * E) Lane {
 //
 // Keys are computed in 32 bits here too, together with a bound of their error, and only a warp that has a value (or a step) within
 // that bound of a border between two codes does it again in 64 bits: the codes are those of the 64-bit computation, which alone took
-// two thirds of the time.  The bound: the sum of squares is 8 + 8 additions deep at most (2^-21 of its root), the reciprocal root is good to 2
-// units (2^-22), two products, and the rotation's two products and sum: less than 2^-20.5 of |a cos| + |b sin| (2^-22.5 without a norm).
+// two thirds of the time.  The bound, in units of 2^-24 of |a cos| + |b sin| (of the value where nothing is rotated): the sum of squares is 8 + 1 + 4
+// additions deep at most and eps one more, which the root halves, 7; the reciprocal root is good to two units in the last place, 4; two products, 2;
+// the rotation's products and sum, 2; and the 64-bit result is rounded to 32 itself, 1.  16, and two more for the products of these errors
+// and what the bound is computed with.  Without a norm 3, of which 4 are made.
 constexpr int kRowWarps = 8, kRowCtas = 2;          // CTAs an SM (three, which leave 80 registers, spill: 100 us for 8 001 tokens of 48 heads instead of 70)
 
 template <typename T>
@@ -323,7 +325,7 @@ write_rows_kernel(const T* qkv, int row_stride, T* q_out, int q_stride, const in
 #pragma unroll
                     for (int e = 0; e < 16; ++e) error = fmaxf(error, fabsf(x[e]));
                 }
-                error *= has_norm ? 6.7434958e-07f : 1.6858740e-07f;       // 2^-20.5, 2^-22.5
+                error *= has_norm ? 1.0728836e-06f : 2.3841858e-07f;       // 18 and 4 times 2^-24
                 if (kind == 1 && rough) error = INFINITY;
             }
         }

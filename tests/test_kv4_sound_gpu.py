@@ -164,3 +164,66 @@ def test_scores_of_far_zero_points(d, new):
         for i in range(new):
             want = values[c["table"][r][0], 0, :i + 2].mean(0)
             assert ((out[c["starts"][r] + i] - want).abs() <= 2.0 ** -8 * 1.01 * (want.abs() + (values[c["table"][r][0], 0, :i + 2].abs().mean(0) if new > 1 else 0))).all(), (r, i)
+
+
+# ---- keys next to the border of two codes ---------------------------------------------------------------------------------------
+
+def rows_whose_roundings_add_up(d, T, nkv, seed):
+    """Keys with one large value whose squares' sum loses nearly half a unit in every addition of a lane's chain, the lanes' exchange and eps:
+    what is computed in 32 bits is above the exact value by as much as it can be.  The rotation's cosines put the normed value within some
+    units of 14.5 steps, the border of two codes."""
+    g = torch.Generator().manual_seed(seed)
+    lanes, nearly = d // 16, 0.99 * 2.0 ** -24
+    rows = torch.zeros(T, nkv, d, dtype=torch.float64)
+    t, h = torch.arange(T)[:, None], torch.arange(nkv)[None]
+    at = torch.randint(0, lanes, (T, nkv), generator=g)                  # the large value: the first of a lane's eight of the first half
+    # sums of squares that reach the large value's lane one exchange after the other
+    share = torch.zeros(T, nkv, lanes, dtype=torch.float64)
+    o, count = lanes // 2, 1
+    while o:
+        for other in range(count):                                       # lanes that the partner at distance o has gathered
+            bits = sum(((other >> i) & 1) * (lanes >> (i + 1)) for i in range(4))
+            share[t, h, at ^ o ^ bits] = nearly / count
+        o, count = o // 2, count * 2
+    rows[..., :] = (share / 16).sqrt().repeat_interleave(8, -1).repeat(1, 1, 2)
+    big = 1 + 0.004 * torch.rand(T, nkv, generator=g, dtype=torch.float64)     # (a unit of its square stays the same)
+    for e in range(8):
+        rows[t, h, 8 * at + e] = nearly ** 0.5 if e else 0.0
+        rows[t, h, d // 2 + 8 * at + e] = (nearly / 8) ** 0.5
+    rows *= big[..., None]
+    rows[t, h, 8 * at] = big
+    return rows.float(), nearly / d
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("norm", [True, False])
+def test_keys_next_to_the_border_of_two_codes(d, norm):
+    """The codes of a long prompt are those of 64 bits and of a call of few tokens, also where the errors of 32 bits add up next to a border."""
+    T, nq, nkv, page = 12000, 1, 2, 16
+    keys, eps = rows_whose_roundings_add_up(d, T, nkv, d)
+    g = torch.Generator().manual_seed(1)
+    gain = (1 + 0.2 * torch.rand(d, generator=g)).to(first.DEV) if norm else None
+    size = 14.5 / (d ** 0.5 * gain.double().cpu()[:d // 2]) if norm else 14.5 / 1.01 * torch.ones(d // 2, dtype=torch.float64)
+    angle = torch.zeros(600, d // 2, 2, dtype=torch.float64)
+    angle[..., 0] = size * 2.0 ** -4 * (1 + (torch.rand(600, d // 2, generator=g, dtype=torch.float64) * 24 - 4) * 2.0 ** -24)
+    table = angle.float().to(first.DEV)
+    if not norm:                                                         # a border for a product of two 24-bit numbers, and its partner's
+        keys = keys * 0 + 2.0 ** -10
+        keys[..., ::8] = 1.01 * (1 + (torch.rand(T, nkv, d // 8, generator=g) * 8 - 4) * 2.0 ** -23)
+        table[..., 1] = table[..., 0] * 2.0 ** -3
+    qkv = torch.cat([torch.zeros(T, nq * d), keys.flatten(1), torch.zeros(T, nkv * d)], 1)
+    positions = torch.arange(T, dtype=torch.int32) % 600
+    pages = T // page + 1
+    cache, small = (torch.zeros(kernels.kv4_cache_shape(pages, nkv, page, d), dtype=torch.uint8, device=first.DEV) for _ in range(2))
+    dev, where, slots = qkv.to(first.DEV), positions.to(first.DEV), first.ints(list(range(T)))
+    q_out = torch.empty(T, nq * d, device=first.DEV)
+    kernels.qk_norm_rope_kv4_write(dev, where, slots, gain, gain, eps if norm else 0.0, table, d, cache, nq, nkv, d, q_out=q_out)
+    for i in range(0, T, 1000):
+        kernels.qk_norm_rope_kv4_write(dev[i:i + 1000], where[i:i + 1000], slots[i:i + 1000], gain, gain, eps if norm else 0.0, table, d, small, nq, nkv, d,
+                                       q_out=q_out[:1000])
+    _, k, _ = first.plain_rows(qkv, positions, gain, gain, eps if norm else 0.0, table, d, nq, nkv, d)
+    want = torch.from_numpy(P4.held(k.numpy().astype(np.float32)))
+    index = torch.arange(T)
+    got, few = (P4.unpack(x, d)[0][index // page, :, index % page] for x in (cache, small))
+    assert torch.equal(few, want)
+    assert torch.equal(got, want), f"{int((got != want).any(-1).sum())} keys differ"
