@@ -150,13 +150,18 @@ class ModelRunner:
     def _activation_bytes(self) -> int:
         """What a step of a full token budget allocates beside weights and cache, and what the captured steps keep
         (each graph has a pool of its own for the intermediates of its sizes); the parts say how much."""
-        step = self.model.workspace_bytes(self.config.max_num_scheduled_tokens, self.config.max_num_seqs)
+        step = self._step_bytes(self.config.max_num_scheduled_tokens)
         if not self.config.enable_cuda_graph:
             return step
         captured = min(self.config.max_num_scheduled_tokens, self.STEP_GRAPH_MAX_TOKENS)
         # the step graphs share one pool, which grows to the largest of them; their results (logits) stay allocated
         logits = self.STEP_GRAPH_LIMIT * 64 * self.vocab_size * 4
-        return step + self.model.workspace_bytes(captured, self.config.max_num_seqs) + logits
+        return step + self._step_bytes(captured) + logits
+
+    def _step_bytes(self, tokens: int) -> int:
+        """What a step of ``tokens`` rows allocates, with the scratch of attention over a cache in 4 bits."""
+        scratch = max((block.mixer.kv4_workspace_bytes(tokens) for block in self.model.blocks), default=0) if self.kv4 else 0
+        return self.model.workspace_bytes(tokens, self.config.max_num_seqs) + scratch
 
     # ---- requests ------------------------------------------------------------------------------------
     def reserve(self, request_id: Hashable, num_new_tokens: int) -> bool:

@@ -982,11 +982,30 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
     _count()
 
 
+KV4_PROMPT_MAX_PARTS = 1 << 24
+_KV4_PROMPT_CTAS = 148               # one an SM
+
+
 def kv4_prompt_shares(ctas: int, keys: int, values: int) -> int:
     """How many CTAs share the keys of a pair of row tiles in the 4-bit prompt attention, for ``ctas`` pairs over all key heads of at most
     ``keys`` keys: as many as the 148 SMs take at once, with 512 keys each at least, and while the partial results (``values`` numbers a
-    share, written and read) stay below 2^24 numbers."""
-    return max(1, min(148 // max(1, ctas), keys // 512, (1 << 24) // max(1, values)))
+    share, written and read) stay below ``KV4_PROMPT_MAX_PARTS`` numbers."""
+    return max(1, min(_KV4_PROMPT_CTAS // max(1, ctas), keys // 512, KV4_PROMPT_MAX_PARTS // max(1, values)))
+
+
+def kv4_attention_scratch_bytes(num_tokens: int, num_q_heads: int, head_dim: int, dtype: torch.dtype) -> int:
+    """Device memory that ``paged_attention_kv4`` allocates at most beside its arguments in a step of up to ``num_tokens`` rows: the partial
+    results of single tokens whose keys are an even list and of prompts whose keys are shared (a mixed step has both)."""
+    if dtype != torch.bfloat16:
+        return 0
+    lib = library()
+    total = 0
+    if lib.cib_attention_kv4_decode_supports(head_dim, KV4_BLOCK):
+        total += 4 * lib.cib_attention_kv4_decode_scratch_floats(head_dim, lib.cib_attention_kv4_decode_ctas(head_dim))
+    if lib.cib_attention_kv4_prompt_supports(head_dim, KV4_BLOCK):
+        rows = min(KV4_PROMPT_MAX_PARTS // head_dim, _KV4_PROMPT_CTAS * num_tokens * num_q_heads)
+        total += 4 * rows * (head_dim + 2)
+    return total
 
 
 def kv4_rows_cluster(ctas: int, keys: int, slots: int) -> int:

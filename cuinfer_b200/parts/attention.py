@@ -91,6 +91,9 @@ class PagedAttention(Mixer):
     def takes_kv4(self, page_size: int) -> bool:
         return kernels.kv4_supports(self.head_dim, page_size)
 
+    def kv4_workspace_bytes(self, tokens: int) -> int:
+        return kernels.kv4_attention_scratch_bytes(tokens, self.num_heads, self.head_dim, self.dtype)
+
     @property
     def capturable(self) -> bool:
         return self.position.capturable

@@ -290,6 +290,10 @@ class Mixer(Part):
         """Whether the mixer writes and reads a paged cache that is held in 4 bits."""
         return False
 
+    def kv4_workspace_bytes(self, tokens: int) -> int:
+        """What ``forward`` allocates in addition to ``workspace_bytes`` where the cache is held in 4 bits."""
+        return 0
+
     def forward(self, x: torch.Tensor, ctx: StepContext, run: int) -> torch.Tensor:
         raise NotImplementedError
 
