@@ -222,7 +222,7 @@ attention_prompt_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
         const int a = folded ? s_pair : 2 * s_pair, b = folded ? row_tiles - 1 - s_pair : 2 * s_pair + 1;
         row0[0] = a * kM, row0[1] = b * kM;
         has[0] = true, has[1] = b < row_tiles && b != a;
-        if (window > 0) k_lo = max(0, seq_len - n + row0[0] / g - window + 1) / kN * kN;
+        if (window > 0) k_lo = max(0, max(0, seq_len - n + row0[0] / g) - window + 1) / kN * kN;       // (a window may be 2^31 - 1)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int last = min(row0[t] + kM, rows_total) - 1;

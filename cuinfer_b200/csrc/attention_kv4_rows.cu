@@ -106,7 +106,7 @@ attention_rows_kernel(const void* __restrict__ q, int bf16, int q_stride, void* 
     const int q0 = query_start_loc[r], n = query_start_loc[r + 1] - q0, seq_len = seq_lens[r];
     const int row0 = s_tile * kRows, rows_total = n * g;
     const int first_pos = seq_len - n + row0 / g, last_pos = seq_len - n + (min(row0 + kRows, rows_total) - 1) / g;
-    int k0 = window > 0 ? max(0, first_pos - window + 1) / kKeys * kKeys : 0;
+    int k0 = window > 0 ? max(0, max(0, first_pos) - window + 1) / kKeys * kKeys : 0;       // (a window may be 2^31 - 1)
     int tiles = last_pos >= k0 ? (last_pos - k0) / kKeys + 1 : 0;
     {
         const int share = (tiles + (int)gridDim.x - 1) / (int)gridDim.x, j0 = (int)blockIdx.x * share;

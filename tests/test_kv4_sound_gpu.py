@@ -227,3 +227,14 @@ def test_keys_next_to_the_border_of_two_codes(d, norm):
     got, few = (P4.unpack(x, d)[0][index // page, :, index % page] for x in (cache, small))
     assert torch.equal(few, want)
     assert torch.equal(got, want), f"{int((got != want).any(-1).sum())} keys differ"
+
+
+# ---- sizes at the ends of what the documentation allows --------------------------------------------------------------------------
+
+@BOTH
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 5, 2 ** 31 - 40])
+def test_the_largest_windows_with_rows_in_front_of_the_first_token(dtype, d, window):
+    """A window of all keys: the rows of a request that brings more tokens than it holds see what they see without one."""
+    c = case([12, 90, 0], [40, 90, 5], 4, 2, d, 16, dtype, window=window, seed=d)
+    check(c)
