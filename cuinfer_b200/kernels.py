@@ -935,7 +935,8 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
         if max(query_lens_host) <= 1:                           # (nothing but single tokens)
             return
         least_query = 2
-    if (dtype == BF16 and lib.cib_attention_kv4_prompt_supports(head_dim, page_size) and scale > 0
+    # (that kernel multiplies masked scores, which are -inf, by the scale: it has to be a positive number in 32 bits too)
+    if (dtype == BF16 and lib.cib_attention_kv4_prompt_supports(head_dim, page_size) and scale > 1e-37
             and q_args[1] % 8 == 0 and q_args[0] % 16 == 0 and out_args[1] % 8 == 0 and out_args[0] % 16 == 0):
         g = num_q_heads // num_kv_heads
         if bound:

@@ -238,3 +238,14 @@ def test_the_largest_windows_with_rows_in_front_of_the_first_token(dtype, d, win
     """A window of all keys: the rows of a request that brings more tokens than it holds see what they see without one."""
     c = case([12, 90, 0], [40, 90, 5], 4, 2, d, 16, dtype, window=window, seed=d)
     check(c)
+
+
+@BOTH
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("scale", [1e-50, 1e-46, 1e-41, 1e-38, 1e-30])
+def test_scales_next_to_zero(dtype, d, new, scale):
+    """A positive scale that is zero in 32 bits, or not a normal number: every key weighs the same, and masked ones nothing."""
+    c = case([90, 70], [new, new], 4, 2, d, 16, dtype, seed=3, window=30)
+    c["scale"] = scale
+    check(c)
