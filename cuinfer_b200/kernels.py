@@ -860,7 +860,10 @@ def qk_norm_rope_kv4_write(qkv: torch.Tensor, positions: torch.Tensor, slot_mapp
 def _row_stride(t: torch.Tensor) -> int:
     """Elements from a row to the next (of a single row: its length, whatever torch calls its stride)."""
     rows, width = t.shape
-    return t.stride(0) if rows > 1 else max(t.stride(0), width)
+    stride = t.stride(0) if rows > 1 else width
+    if stride >= 1 << 31:
+        raise KernelError(f"rows {stride} elements apart do not fit 32-bit strides")
+    return stride
 
 
 def kv4_read(cache: torch.Tensor, slots: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, num_kv_heads: int, head_dim: int) -> None:
@@ -906,6 +909,9 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
         raise KernelError(f"{who}: window and max_seq_len must not be negative, nor 2^31 or more")
     if block_table.dtype is not torch.int32:
         raise KernelError(f"{who}: block_table must be torch.int32, got {block_table.dtype}")
+    out_stride = _row_stride(out)
+    if out_stride < width:
+        raise KernelError(f"{who}: rows of out that are {out_stride} values apart hold no {width} each")
     _same_device(who, q, out, cache, block_table, query_start_loc, seq_lens)
     if T == 0 or R == 0:
         return
@@ -913,7 +919,7 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
     cache_args = (_dense(cache, "cache"), cache.shape[0], page_size, block_table.data_ptr(), _row_stride(block_table), block_table.shape[1],
                   _dense(query_start_loc, "query_start_loc", torch.int32), _dense(seq_lens, "seq_lens", torch.int32))
     q_args = (q.data_ptr(), _row_stride(q))
-    out_args = (out.data_ptr(), _row_stride(out))
+    out_args = (out.data_ptr(), out_stride)
     dtype = _code(q, "q")
     pdl = 1 if use_pdl else 0
     bound = sum(query_lens_host) > T

@@ -50,3 +50,37 @@ def test_no_launch_needs_more_scratch():
             shares = kernels.kv4_prompt_shares((-(-T * g // 256)) * nkv, keys, T * nq * d)
             used += 4 * shares * T * nq * (d + 2) if shares > 1 else 0
         assert used <= kernels.kv4_attention_scratch_bytes(budget, nq, d, torch.bfloat16)
+
+
+# ---- calls that are refused -------------------------------------------------------------------------------------------------------
+
+def attention_args(**change):
+    args = dict(q=torch.zeros(3, 256), out=torch.zeros(3, 256), cache=torch.zeros(kernels.kv4_cache_shape(2, 2, 16, 64), dtype=torch.uint8),
+                block_table=torch.zeros(2, 1, dtype=torch.int32), query_start_loc=torch.tensor([0, 1, 3], dtype=torch.int32),
+                seq_lens=torch.tensor([1, 2], dtype=torch.int32), query_lens_host=[1, 2], num_q_heads=4, num_kv_heads=2, head_dim=64,
+                scale=0.125, max_seq_len=2)
+    return {**args, **change}
+
+
+def far_apart(rows, width, stride, dtype=torch.float32):
+    return torch.empty_strided((rows, width), (stride, 1), dtype=dtype, device="meta")
+
+
+@pytest.mark.parametrize("change, match", [
+    (dict(out=torch.zeros(1, 256).expand(3, 256)), "apart"),
+    (dict(out=torch.zeros(1000).as_strided((3, 256), (255, 1))), "apart"),
+    (dict(out=far_apart(3, 256, 1 << 31)), "32-bit strides"),
+    (dict(out=far_apart(3, 256, 1 << 33)), "32-bit strides"),
+])
+def test_attention_refuses_rows_that_overlap_or_lie_too_far_apart(change, match):
+    with pytest.raises(kernels.KernelError, match=match):
+        kernels.paged_attention_kv4(**attention_args(**change))
+
+
+def test_strides_of_rows():
+    """32 bits of a stride go to the kernels; of a single row nothing does."""
+    assert kernels._row_stride(far_apart(2, 64, (1 << 31) - 8)) == (1 << 31) - 8
+    assert kernels._row_stride(far_apart(1, 64, 1 << 40)) == 64 and kernels._row_stride(torch.zeros(5, 3, 64)[:, 1]) == 192
+    for stride in (1 << 31, (1 << 32) + 64):
+        with pytest.raises(kernels.KernelError, match="32-bit strides"):
+            kernels._row_stride(far_apart(2, 64, stride))
