@@ -249,3 +249,67 @@ def test_scales_next_to_zero(dtype, d, new, scale):
     c = case([90, 70], [new, new], 4, 2, d, 16, dtype, seed=3, window=30)
     c["scale"] = scale
     check(c)
+
+
+@BOTH
+@pytest.mark.parametrize("heads", [(300, 1, 64), (130, 1, 128), (70, 1, 96), (9, 1, 256), (258, 2, 32)])
+def test_many_query_heads_to_a_key_head(dtype, heads):
+    """A token's heads fill more than a row tile."""
+    nq, nkv, d = heads
+    check(case([70, 33, 5, 128], [3, 1, 5, 1], nq, nkv, d, 16, dtype, seed=d, spare_rows=1))
+
+
+@BOTH
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("lens", ["exact", "bounds"])
+def test_a_hundred_requests_of_every_kind(dtype, d, lens):
+    rng = random.Random(d)
+    new = [rng.choice([0, 1, 1, 2, 17, 40]) for _ in range(101)]
+    lengths = [n + rng.choice([0, 3, 60]) for n in new]
+    c = case(lengths, new, 4, 2, d, 16, dtype, seed=d, spare_rows=2)
+    check(c, attend(c, lens=None if lens == "exact" else [sum(new) + 128] + [1] * 100, longest=None if lens == "exact" else 3000))
+
+
+@BOTH
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("new", [1, 9])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_query_that_is_no_number_is_its_own_rows_business(dtype, d, new, bad):
+    c = case([60, 300], [new, new], 6, 2, d, 16, dtype, seed=d)
+    clean = attend(c).clone().reshape(2, new, 6, d)
+    q = c["q"].clone()
+    q[0, 1 * d + 7] = bad                                                # request 0, its first row, head 1
+    q[new, 4 * d] = bad                                                  # request 1, its first row, head 4
+    c["q"] = q
+    got = attend(c, torch.full_like(c["out"], 5.0)).reshape(2, new, 6, d)
+    for r, head in ((0, 1), (1, 4)):
+        assert torch.isnan(got[r, 0, head]).all()
+        got[r, 0, head] = clean[r, 0, head]
+    assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_recorded_step_of_a_long_model_for_any_batch(d):
+    """One graph with the bounds of a recorded step and the longest context of its model, replayed for batches with and without single tokens, with
+    requests that bring nothing, and with rows that belong to none of them."""
+    R, T = 9, 96
+    batches = [[40, 30, 0, 1, 2, 20, 3, 0, 0], [1] * 9, [96, 0, 0, 0, 0, 0, 0, 0, 0], [2, 3, 4, 5, 6, 7, 8, 9, 10], [0] * 9, [1, 0, 60, 0, 0, 0, 0, 1, 0]]
+    c = case([400] * R, [T // R] * R, 4, 2, d, 16, BF16, seed=d, spare_rows=T - R * (T // R))
+    table, starts, lengths = first.ints(c["table"]), first.ints([0] * (R + 1)), first.ints([0] * R)
+
+    def call():
+        kernels.paged_attention_kv4(c["q"], c["out"], c["cache"], table, starts, lengths, [T + 128] + [1] * (R - 1), 4, 2, d, c["scale"], max_seq_len=40960)
+
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    rng = random.Random(d)
+    for new in batches + batches[::-1]:
+        c["new"], c["lengths"] = new, [n + rng.randrange(400 - n) if n else 0 for n in new]
+        c["starts"] = [sum(new[:i]) for i in range(R + 1)]
+        starts.copy_(first.ints(c["starts"]))
+        lengths.copy_(first.ints(c["lengths"]))
+        c["out"].fill_(5.0)
+        graph.replay()
+        check(c, c["out"])
