@@ -139,7 +139,7 @@ class ModelRunner:
         # room for a step's activations: qkv/gate_up/logits rows of a full token budget
         budget -= self._activation_bytes()
         per_page = max(1, self.page_bytes())
-        pages = budget // per_page
+        pages = min(budget // per_page, ((1 << 31) - 1) // self.page_size)       # (slots are numbered in 32 bits)
         need = (self.max_model_len + self.page_size - 1) // self.page_size
         if pages < need:
             raise RuntimeError(

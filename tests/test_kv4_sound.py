@@ -84,3 +84,18 @@ def test_strides_of_rows():
     for stride in (1 << 31, (1 << 32) + 64):
         with pytest.raises(kernels.KernelError, match="32-bit strides"):
             kernels._row_stride(far_apart(2, 64, stride))
+
+
+def test_a_pool_has_no_more_slots_than_32_bits_number(monkeypatch):
+    """One key head of 32 in one layer: 180 GB would be some 4e9 slots of 36 bytes."""
+    cfg = dict(TINY_B, num_hidden_layers=1, num_attention_heads=2, num_key_value_heads=1)
+    for kv4, block in ((True, 16), (True, 48), (False, 16)):
+        runner = runner_without_a_device(cfg, torch.bfloat16, kv4, block_size=block)
+        from cuinfer_b200.cache import group_runs
+        runner.groups = group_runs(runner.model.cache_needs())
+        runner.page_size, runner.dtype, runner.device, runner.max_model_len = block, torch.bfloat16, "cuda:0", 768
+        monkeypatch.setattr(torch.cuda, "mem_get_info", lambda device: (180 << 30, 180 << 30))
+        pages = runner._pages_from_memory()
+        assert 0 < pages * block < 1 << 31
+        if not kv4:
+            assert pages * runner.page_bytes() > 140 << 30               # (128 bytes a slot: the memory ends first)
