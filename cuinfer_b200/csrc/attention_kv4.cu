@@ -8,7 +8,8 @@
 // head (a key is taken apart once for all four); its warps share the keys in chunks of 32, a key to a lane for the scores, a value
 // column to a lane for the weighted sum, and merge their running maxima and sums in shared memory.  Where that leaves SMs without work, a
 // cluster of up to eight CTAs shares the keys and joins its parts through distributed shared memory: one token of 4 000 keys, 16 heads over 8 of
-// 128, takes 31 us (45 with conversions of integers and a value at a time, 270 without clusters), 64 of them 424; bound by issue.  32-bit throughout,
+// 128, takes 31 us (45 with conversions of integers and a value at a time, 270 without clusters), 64 of them 424, most of it taking every code apart for
+// two heads.  32-bit throughout,
 // the exact exponential; nothing is rounded before the end.  Keys whose page the block table does not name are left out; a row
 // without keys is zero; rows that belong to no request are left as they are.
 #include "kv4.cuh"

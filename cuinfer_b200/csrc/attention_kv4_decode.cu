@@ -367,8 +367,8 @@ attention_decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_
                 }
         }
     };
-    // ---- O += (p step) (code - zero) of a stage.  p enters as two bfloat16 parts, so that only p * step is rounded (2^-9 of it; what the parts
-    // leave out is 2^-18) ----
+    // ---- O += (p step) (code - zero) of a stage.  p enters as two bfloat16 parts, so that only p * step is rounded (2^-8 of it; what the parts
+    // leave out is 2^-16) ----
     auto values = [&](const unsigned char* stage, const uint32_t (&ph)[2][2], const uint32_t (&pl)[2][2]) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {

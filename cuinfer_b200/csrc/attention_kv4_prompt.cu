@@ -11,7 +11,7 @@
 //   * S = Q K^T and O += P V are `tcgen05.mma.cta_group::1.kind::f16`, S, P and O in tensor memory (2 x (64 + 64 + 128) columns), issued by one
 //     thread; S of key tile j + 1 is computed while the softmax warps take the exponentials of tile j.
 //   * Eight softmax warps, a thread per row: running maximum in base 2 that is raised when it grows by more than 8 (or at all over the
-//     first 256 keys); P goes back over its scores in bfloat16, which rounds each weight once (2^-9 of it), the sum is of the weights before that.
+//     first 256 keys); P goes back over its scores in bfloat16, which rounds each weight once (2^-8 of it), the sum is of the weights before that.
 //   * Rows see the keys up to their position, the last `window` of them, and none of a page that the block table does not name.  A value that is not
 //     a number must not reach rows that do not see its key (0 x NaN is NaN): it is written as zero, and where a CTA has met one, its rows look
 //     through the words of the values that they see at the end.

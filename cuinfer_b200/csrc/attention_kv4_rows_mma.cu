@@ -5,7 +5,7 @@
 // tile's keys and values apart once for all rows, from words that were asked for a tile ahead, into shared memory as bfloat16 numbers (step * (code - zero)
 // is exact): keys as [key][column], values transposed, [column][key], because a word of value codes holds two neighbouring keys of a column and
 // the second product sums over keys.  Scores stay in registers; in the layout in which m16n8k16 leaves them they are the first operand of the second
-// product: p is rounded to bfloat16 once (2^-9 of it), the sum is of the weights before that.  32-bit running maximum and sum per row.
+// product: p is rounded to bfloat16 once (2^-8 of it), the sum is of the weights before that.  32-bit running maximum and sum per row.
 //
 // Bound by the latency of a tile's steps (four warps, two CTAs an SM) and mma.sync's rate.  2 x 400 tokens behind 1 600, 8 heads of 256 over 2: 637 us by
 // 32-bit multiply-adds, 158 so; 8 heads of 96 262 and 63.

@@ -823,7 +823,9 @@ def qk_norm_rope_kv4_write(qkv: torch.Tensor, positions: torch.Tensor, slot_mapp
     """``qk_norm_rope_kv_write`` for a cache held in 4 bits (``kv4_cache_shape``): per-head RMSNorm (if weights are given) and rotary
     encoding (if a table is given) of the query and key heads of the packed ``qkv`` rows; keys and values are quantised in
     groups of 32 values and appended to the slots ``slot_mapping`` (-1: none; no slot twice in a call).  The queries go to
-    ``q_out`` [T, nq*d], or replace those of ``qkv`` where none is given; keys and values of ``qkv`` stay as they are."""
+    ``q_out`` [T, nq*d], or replace those of ``qkv`` where none is given; keys and values of ``qkv`` stay as they are.
+    Positions, slots, gains and the table are read while the kernel in front may still run, where that kernel lets the next one start early (those of this
+    module do): they are not its results."""
     who = "qk_norm_rope_kv4_write"
     if qkv.dim() != 2 or qkv.stride(1) != 1:
         raise KernelError(f"{who}: qkv must be [T, (nq + 2 nkv) * d] with dense rows")
@@ -890,8 +892,9 @@ def paged_attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor,
     are row r of ``block_table`` (a page that is none, -1, or behind the row's end: its keys are left out).  ``window`` > 0: a query sees the last so many
     keys.  Rows that see no key are zero; rows behind the last request are left as they are.  ``query_lens_host``: how many rows
     each request brings (host ints, or an upper bound as ``StepContext.query_lens_for_launch`` gives); ``max_seq_len``: no request
-    has more keys.  Both shape the launch only.  ``out`` shares no memory with ``q``.  float32 or bfloat16; in bfloat16 queries and
-    what the cache holds are below 2^120 in magnitude (steps are scaled by powers of two on the way)."""
+    has more keys.  Both shape the launch only.  ``out`` shares no memory with ``q``.  float32 or bfloat16; scores and sums are 32-bit
+    numbers in both, and in bfloat16 queries and what the cache holds are below 2^120 in magnitude (steps are scaled by powers of two on the way).
+    ``query_start_loc`` and ``seq_lens`` are no results of the kernel in front where that one lets the next start early (``qk_norm_rope_kv4_write``)."""
     who = "paged_attention_kv4"
     T = q.shape[0]
     page_size = _kv4_cache(cache, num_kv_heads, head_dim, who)
